@@ -9,8 +9,9 @@
  *
  * Part 1 is the reference's own ABI, same names, argument meaning and error
  * behaviour, so existing ctypes/cgo bindings load this library unchanged.
- * Parts 2-4 are additions (batched sessions, device-resident session pools and
- * the isolated spiking-network tick engine); they follow the same conventions.
+ * Parts 2-5 are additions (batched sessions, device-resident session pools, the
+ * isolated spiking-network tick engine and decoding operators); they follow the
+ * same conventions.
  */
 #ifndef NEUROGEN_B200_H
 #define NEUROGEN_B200_H
@@ -120,6 +121,18 @@ int ng_pool_step_device(void *pool, const int *d_tokens, float *d_logits,
                         void *stream);
 /* Device pointer to the pool's state [batch, state_size]. */
 float *ng_pool_device_state(void *pool);
+/* CUDA device the pool's sessions live on. */
+int ng_pool_device(void *pool);
+/* Reports an error that a kernel of an enqueued step recorded (a bounded wait
+ * that ran out); call it after synchronising with the step's stream. */
+int ng_pool_check(void *pool);
+/* Beam search: the pool's sessions in groups of `beams` (1..32, dividing the
+ * pool); session w of each group takes over the state of session parents[.][w]
+ * of its group (ng_state_reorder on the pool's state).  Host parents [batch],
+ * checked, and synchronous; or device parents on a caller stream (NULL = the
+ * engine's), enqueued only. */
+int ng_pool_reorder(void *pool, int beams, const int32_t *parents);
+int ng_pool_reorder_device(void *pool, int beams, const int32_t *d_parents, void *stream);
 
 /* ------------------------------------------------------------------------ */
 /* Part 4: isolated-tick spiking network (conductance ALIF + delay ring).    */
@@ -291,6 +304,69 @@ int ng_net_plasticity_state(void *net, float *pre_trace, float *potential_trace,
  * copies, no synchronisation.  d_spikes/d_counts may be NULL. */
 int ng_net_run_device(void *net, int ticks, uint32_t *d_spikes,
                       int64_t *d_counts, void *stream);
+
+/* ------------------------------------------------------------------------ */
+/* Part 5: decoding operators on device buffers.                             */
+/* ------------------------------------------------------------------------ */
+
+/* Every call takes the device its arrays live on and a stream of that device
+ * (cudaStream_t as void*; NULL = the default stream), enqueues its work there,
+ * and returns without synchronising; the caller's current device stays as it
+ * is.  Nothing is allocated, and nothing is kept between calls.  Calls can be
+ * captured into CUDA graphs once the same call has run outside one. */
+
+/* Element types of 16- and 32-bit arrays. */
+enum { NG_F32 = 0, NG_BF16 = 1, NG_F16 = 2 };
+
+/* 8-bit block-scaled matrices: e4m3 bytes, one fp32 scale for each block of
+ * 128 columns and block_rows rows (1: activations, 128: weights), scales
+ * row-major [ceil(rows / block_rows)][ceil(cols / 128)]; a value stands for
+ * byte * scale.  8-bit rows start on 16-byte boundaries (address and stride).
+ *
+ * scale = max(amax |x| / 448, 2^-126), byte = e4m3(x / scale), both divisions
+ * rounded to fp32 and the byte to nearest even.  A block with a NaN has a NaN
+ * scale and one with an infinity an infinite scale, so that products with it
+ * are NaN.  x: rows of cols elements, row stride ldx elements. */
+int ng_block_quantize(int device, const void *x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int block_rows,
+                      void *q, int64_t ldq, float *scale, void *stream);
+
+/* y[m][n] = sum_k a[m][k] w[n][k] (+ bias[n]) (+ add_scale * add[m][n]), a with
+ * a scale for each 1 x 128 block, w for each 128 x 128 block.  fp32 sums: the
+ * bytes' products of one block of 128 on the tensor cores, then the blocks in
+ * a fixed order; rounded once to y's type.  The result is a function of the
+ * operands and sizes alone.  bias and add are fp32 and may be NULL; y may be
+ * add when it is fp32 with the same stride. */
+int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale, const void *w, int64_t ldw,
+                    const float *w_scale, int64_t m, int64_t n, int64_t k, const float *bias, const float *add,
+                    int64_t ldadd, float add_scale, void *y, int dtype, int64_t ldy, void *stream);
+
+/* Beam search's step for `groups` searches of `beams` (1..32) beams: logits
+ * [groups * beams] rows of vocab (row stride ld elements), scores [groups][beams]
+ * the beams' cumulative log probabilities (-inf: no such beam), finished
+ * [groups][beams] 0/1 or NULL, allowed [vocab] 0/1 or NULL.
+ *
+ * Beam w's candidate of allowed token v scores scores[w] + log softmax(logits[w])[v],
+ * the softmax over the allowed tokens; a finished beam has one candidate, token
+ * `pad` at its own score.  The best `beams` candidates, best first, become
+ * next_scores, tokens, parents (the beam within the group) and next_finished
+ * (the parent's, or the token is `end`; end < 0: no token ends a beam).  Scores
+ * are formed in 64 bits and rounded once; a beam's equal logits go to the lower
+ * token, equal scores of two beams to the lower beam.  A candidate whose score
+ * is not finite is none (a row whose mask leaves nothing, or that holds a NaN
+ * or +inf at an allowed token, has none); slots that no candidate fills get
+ * score -inf, `pad`, their own index as parent, and count as finished.
+ * next_scores may be scores and next_finished may be finished. */
+size_t ng_beam_workspace(int groups, int beams, int vocab);
+int ng_beam_select(int device, const void *logits, int dtype, int64_t ld, int groups, int beams, int vocab,
+                   const float *scores, const uint8_t *finished, const uint8_t *allowed, int end, int pad,
+                   float *next_scores, int32_t *tokens, int32_t *parents, uint8_t *next_finished, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/* Rows of row_bytes at a stride of ld_bytes, beams (1..32) rows a group:
+ * row [g][w] becomes the old row [g][parents[g][w]], in place.  A parent
+ * outside 0..beams-1 leaves its row as it was. */
+int ng_state_reorder(int device, void *states, int64_t row_bytes, int64_t ld_bytes, int groups, int beams,
+                     const int32_t *parents, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,50 @@
+// 8-bit block-scaled operands: quantisation and product (block_quant.cu,
+// block_matmul.cu).  A matrix [rows][cols] is held as e4m3 bytes, row stride a
+// multiple of 16 bytes, with one fp32 scale for each block of 128 columns and
+// `block` rows (1 for activations, 128 for weights), scales row-major
+// [ceil(rows / block)][ceil(cols / 128)].
+#pragma once
+#include <cuda_runtime.h>
+#include <cstdint>
+
+namespace ngb {
+
+constexpr int kScaleBlock = 128;
+
+// Element types of the operators' 16- and 32-bit arrays (NG_F32, NG_BF16, NG_F16).
+enum class Elem : int { f32 = 0, bf16 = 1, f16 = 2 };
+inline size_t elem_size(Elem t) { return t == Elem::f32 ? 4 : 2; }
+
+struct QuantArgs {
+  const void *x; // [rows] rows of cols, row stride ldx elements
+  Elem type;
+  const int *xidx; // optional row gather: row r of the result comes from row xidx[r] of x
+  long rows, cols, ldx;
+  int block; // rows a scale covers: 1 or 128
+  uint8_t *q;
+  long ldq; // bytes
+  float *scale;
+};
+void launch_block_quantize(const QuantArgs &a, cudaStream_t s);
+
+// y[m][n] = sum_b a_scale[m][b] w_scale[n / 128][b] sum_{k in block b} a[m][k] w[n][k]
+//           + bias[n] + add_scale * add[m][n]
+struct BlockMatmulArgs {
+  const uint8_t *a;
+  long lda;
+  const float *a_scale;
+  const uint8_t *w;
+  long ldw;
+  const float *w_scale;
+  const float *bias; // [n] or null
+  const float *add;  // [m] rows of n or null
+  long ldadd;
+  float add_scale;
+  void *y;
+  Elem type;
+  long ldy;
+  int m, n, k;
+};
+void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s);
+
+} // namespace ngb

@@ -2,6 +2,7 @@
 // convention as the reference's C ABI (src/native/NeuralEngine.cpp:193-267):
 // exceptions become -1 / NULL plus a thread-local ng_error() message, and one
 // mutex per engine serialises calls on a shared handle.
+#include "beam_kernels.h"
 #include "capi_common.h"
 #include "lang_engine.h"
 #include "neurogen_b200.h"
@@ -28,7 +29,7 @@ NeuralEngine &checked(void *p, const float *state, size_t n) {
 struct Pool {
   NeuralEngine *engine;
   int B;
-  DeviceBuffer state, tokens, logits, hidden, act;
+  DeviceBuffer state, tokens, logits, hidden, act, parents;
   Scratch sc;
   cudaStream_t stream = nullptr;
   cudaGraphExec_t graph = nullptr; // one token step of the whole pool
@@ -59,6 +60,16 @@ struct Pool {
       cuda_check(e, "cudaGraphInstantiate");
     }
     NGB_CUDA(cudaGraphLaunch(graph, st));
+  }
+  void check_beams(int beams) const {
+    if (beams < 1 || beams > kMaxBeams) throw std::invalid_argument("Beams must be 1..32");
+    if (B % beams) throw std::invalid_argument("Beams must divide the pool's sessions");
+  }
+  // Session w of each group of `beams` takes over the state of session d_parents[.][w].
+  void reorder(int beams, const int *d_parents, cudaStream_t st) {
+    const long row = long(engine->state_size()) * 4;
+    launch_state_reorder({state.as<void>(), row, row, B / beams, beams, d_parents}, st);
+    NGB_CUDA(cudaGetLastError());
   }
 };
 } // namespace
@@ -147,6 +158,7 @@ void *ng_pool_create(void *engine, int batch) {
     pool->logits.reset(size_t(batch) * kVocab * 4);
     pool->hidden.reset(size_t(batch) * e->config.width * 4);
     pool->act.reset(size_t(batch) * 4);
+    pool->parents.reset(size_t(batch) * sizeof(int));
     pool->sc.ensure(m.dims, batch, m.tc_proj);
     NGB_CUDA(cudaStreamCreateWithFlags(&pool->stream, cudaStreamNonBlocking));
     return pool.release();
@@ -220,6 +232,42 @@ int ng_pool_step_device(void *p, const int *d_tokens, float *d_logits, void *str
   });
 }
 
+int ng_pool_reorder(void *p, int beams, const int32_t *parents) {
+  return guarded([&] {
+    if (!p || !parents) throw std::invalid_argument("Null pool or parents");
+    auto &pool = *static_cast<Pool *>(p);
+    std::lock_guard<std::mutex> lock(pool.mu);
+    pool.check_beams(beams);
+    for (int b = 0; b < pool.B; ++b)
+      if (parents[b] < 0 || parents[b] >= beams) throw std::invalid_argument("Parents must be beams of the same group");
+    NGB_CUDA(cudaSetDevice(pool.engine->device().device));
+    NGB_CUDA(cudaMemcpyAsync(pool.parents.as<int>(), parents, pool.B * sizeof(int), cudaMemcpyHostToDevice,
+                             pool.stream));
+    pool.reorder(beams, pool.parents.as<int>(), pool.stream);
+    NGB_CUDA(cudaStreamSynchronize(pool.stream));
+  });
+}
+
+int ng_pool_reorder_device(void *p, int beams, const int32_t *d_parents, void *stream) {
+  return guarded([&] {
+    if (!p || !d_parents) throw std::invalid_argument("Null pool or parents");
+    auto &pool = *static_cast<Pool *>(p);
+    std::lock_guard<std::mutex> lock(pool.mu);
+    pool.check_beams(beams);
+    NGB_CUDA(cudaSetDevice(pool.engine->device().device));
+    pool.reorder(beams, d_parents, stream ? static_cast<cudaStream_t>(stream) : pool.stream);
+  });
+}
+
 float *ng_pool_device_state(void *p) { return p ? static_cast<Pool *>(p)->state.as<float>() : nullptr; }
+
+int ng_pool_check(void *p) {
+  return guarded([&] {
+    if (!p) throw std::invalid_argument("Null pool");
+    static_cast<Pool *>(p)->engine->device().check_device_errors();
+  });
+}
+
+int ng_pool_device(void *p) { return p ? static_cast<Pool *>(p)->engine->device().device : -1; }
 
 } // extern "C"

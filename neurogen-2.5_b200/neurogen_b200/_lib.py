@@ -30,7 +30,8 @@ EXPORTS = (
     'ng_net_run_device', 'ng_topology_create', 'ng_topology_destroy', 'ng_topology_synapses',
     'ng_topology_export', 'ng_net_create_topology', 'ng_net_stats', 'ng_step_static', 'ng_net_launch_kind',
     'ng_net_create_partitioned', 'ng_nccl_unique_id', 'ng_math_eval', 'ng_net_plasticity_state',
-    'ng_net_exchange_kind',
+    'ng_net_exchange_kind', 'ng_pool_reorder', 'ng_pool_reorder_device', 'ng_pool_device', 'ng_pool_check',
+    'ng_block_quantize', 'ng_block_matmul', 'ng_beam_workspace', 'ng_beam_select', 'ng_state_reorder',
 )
 
 
@@ -111,6 +112,25 @@ def library():
     lib.ng_pool_step_device.restype = ci
     lib.ng_pool_device_state.argtypes = [vp]
     lib.ng_pool_device_state.restype = vp
+    lib.ng_pool_reorder.argtypes = [vp, ci, I32]
+    lib.ng_pool_reorder.restype = ci
+    lib.ng_pool_reorder_device.argtypes = [vp, ci, vp, vp]
+    lib.ng_pool_reorder_device.restype = ci
+    lib.ng_pool_device.argtypes = [vp]
+    lib.ng_pool_device.restype = ci
+    lib.ng_pool_check.argtypes = [vp]
+    lib.ng_pool_check.restype = ci
+    i64, cf = ct.c_int64, ct.c_float
+    lib.ng_block_quantize.argtypes = [ci, vp, ci, i64, i64, i64, ci, vp, i64, vp, vp]
+    lib.ng_block_quantize.restype = ci
+    lib.ng_block_matmul.argtypes = [ci, vp, i64, vp, vp, i64, vp, i64, i64, i64, vp, vp, i64, cf, vp, ci, i64, vp]
+    lib.ng_block_matmul.restype = ci
+    lib.ng_beam_workspace.argtypes = [ci, ci, ci]
+    lib.ng_beam_workspace.restype = sz
+    lib.ng_beam_select.argtypes = [ci, vp, ci, i64, ci, ci, ci, vp, vp, vp, ci, ci, vp, vp, vp, vp, vp, sz, vp]
+    lib.ng_beam_select.restype = ci
+    lib.ng_state_reorder.argtypes = [ci, vp, i64, i64, ci, ci, vp, vp]
+    lib.ng_state_reorder.restype = ci
     cfgp = ct.POINTER(NetConfig)
     lib.ng_net_default_config.argtypes = [cfgp]
     lib.ng_net_default_config.restype = None
@@ -160,6 +180,21 @@ def library():
 
 def error():
     return library().ng_error().decode()
+
+
+F32_CODE = 0   # NG_F32
+
+
+def check(code):
+    """Raise the library's error text when an entry point reports a failure."""
+    if code:
+        raise ValueError(error())
+
+
+def stream_of(device):
+    """Address of the current torch stream of a CUDA device."""
+    import torch
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def ptr(array):

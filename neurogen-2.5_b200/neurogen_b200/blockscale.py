@@ -1,0 +1,106 @@
+"""8-bit block-scaled matrices on the GPU (include/neurogen_b200.h part 5).
+
+A matrix is e4m3 bytes with one fp32 scale for each block of 128 columns and one row
+(activations) or 128 rows (weights).  ``matmul`` multiplies two of them on the tensor cores; the
+engine's opt-in 8-bit projections (``NEUROGEN_PROJECTION=fp8``) are these operators.  They take
+CUDA tensors, run on the current stream of the tensors' device and do not synchronise; nothing
+is kept between calls.  Inference only: no gradients flow through them.
+"""
+import torch
+
+from ._lib import library, F32_CODE, check, stream_of
+
+BLOCK = 128
+ELEMENTS = {torch.float32: F32_CODE, torch.bfloat16: 1, torch.float16: 2}
+E4M3 = torch.float8_e4m3fn
+
+
+def _matrix(x, what):
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise ValueError(f'{what} must be a tensor [rows, columns]')
+    if x.device.type != 'cuda':
+        raise ValueError(f'{what} must be on a CUDA device; there is no CPU fallback')
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        raise ValueError(f'{what} must have adjacent columns')
+    return x.shape
+
+
+def _row_stride(x):
+    """Elements from a row to the next; a single row has no next."""
+    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], x.stride(0))
+
+
+def _stride16(x):
+    """Row stride of an 8-bit matrix; a single row takes the next multiple of 16."""
+    return x.stride(0) if x.shape[0] > 1 else -(-x.shape[1] // 16) * 16
+
+
+def _vector(x, shape, dtype, device, what):
+    if (not isinstance(x, torch.Tensor) or x.shape != shape or x.dtype != dtype or x.device != device
+            or not x.is_contiguous()):
+        raise ValueError(f'{what} must be contiguous {dtype} {list(shape)} on {device}')
+
+
+def quantize(x, rows=1):
+    """``x`` [m, k] (float32, bfloat16 or float16) as (e4m3 [m, k], scale): a scale for each 1 x 128
+    block (``rows=1``) or 128 x 128 block (``rows=128``).
+
+    scale = max(amax / 448, 2^-126) and byte = e4m3(x / scale), rounded to nearest even.  The bytes'
+    rows start on 16-byte boundaries (their row stride is k rounded up to 16).
+    """
+    m, k = _matrix(x, 'x')
+    if x.dtype not in ELEMENTS:
+        raise ValueError('x must be float32, bfloat16 or float16')
+    if rows not in (1, BLOCK):
+        raise ValueError('A scale covers 1 or 128 rows')
+    if k < 1:
+        raise ValueError('x must have at least one column')
+    device = x.device
+    ldq = -(-k // 16) * 16
+    q = torch.empty_strided((m, k), (ldq, 1), dtype=E4M3, device=device)
+    scale = torch.empty((-(-m // rows), -(-k // BLOCK)), dtype=torch.float32, device=device)
+    check(library().ng_block_quantize(device.index, x.data_ptr(), ELEMENTS[x.dtype], m, k, _row_stride(x), rows,
+                                      q.data_ptr(), ldq, scale.data_ptr(), stream_of(device)))
+    return q, scale
+
+
+def matmul(a, a_scale, w, w_scale, bias=None, add=None, add_scale=1.0, out_dtype=torch.float32):
+    """``a @ w.T`` (+ ``bias``) (+ ``add_scale * add``) of two block-scaled matrices.
+
+    ``a`` e4m3 [m, k] with scales for 1 x 128 blocks, ``w`` e4m3 [n, k] with scales for 128 x 128
+    blocks (``quantize(w, 128)``); rows on 16-byte boundaries.  ``bias`` float32 [n], ``add``
+    float32 [m, n].  fp32 sums, rounded once to ``out_dtype`` (float32, bfloat16 or float16).
+    """
+    m, k = _matrix(a, 'a')
+    n, kw = _matrix(w, 'w')
+    if a.dtype != E4M3 or w.dtype != E4M3:
+        raise ValueError('a and w must be float8_e4m3fn')
+    if kw != k:
+        raise ValueError(f'a has {k} columns and w {kw}')
+    if k < 1 or n < 1:
+        raise ValueError('w must not be empty')
+    if out_dtype not in ELEMENTS:
+        raise ValueError('out_dtype must be float32, bfloat16 or float16')
+    device = a.device
+    if w.device != device:
+        raise ValueError('a and w must be on the same device')
+    kb = -(-k // BLOCK)
+    _vector(a_scale, (m, kb), torch.float32, device, 'a_scale')
+    _vector(w_scale, (-(-n // BLOCK), kb), torch.float32, device, 'w_scale')
+    if bias is not None:
+        _vector(bias, (n,), torch.float32, device, 'bias')
+    if add is not None and (_matrix(add, 'add') != (m, n) or add.dtype != torch.float32 or add.device != device):
+        raise ValueError(f'add must be float32 [{m}, {n}] on {device}')
+    y = torch.empty((m, n), dtype=out_dtype, device=device)
+    check(library().ng_block_matmul(device.index, a.data_ptr(), _stride16(a), a_scale.data_ptr(), w.data_ptr(),
+                                    _stride16(w), w_scale.data_ptr(), m, n, k,
+                                    None if bias is None else bias.data_ptr(),
+                                    None if add is None else add.data_ptr(),
+                                    n if add is None else _row_stride(add), add_scale, y.data_ptr(),
+                                    ELEMENTS[out_dtype], n, stream_of(device)))
+    return y
+
+
+def linear(x, w, w_scale, bias=None, add=None, add_scale=1.0, out_dtype=torch.float32):
+    """``quantize(x)`` times the block-scaled weights ``w``: a projection in 8 bits."""
+    return matmul(*quantize(x), w, w_scale, bias, add, add_scale, out_dtype)

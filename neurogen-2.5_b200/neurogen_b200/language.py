@@ -424,6 +424,18 @@ def load_session(path, checkpoint_id):
     return payload
 
 
+def trace_beams(tokens, parents):
+    """Sequences [groups, beams, steps] of a beam search from each step's chosen tokens and parents
+    [steps, groups, beams]: a beam's last token is its own, the one before its parent's, and so on."""
+    steps, groups, beams = tokens.shape
+    out = np.empty((groups, beams, steps), np.int32)
+    slot = np.broadcast_to(np.arange(beams), (groups, beams))
+    for t in range(steps - 1, -1, -1):
+        out[:, :, t] = np.take_along_axis(tokens[t], slot, 1)
+        slot = np.take_along_axis(parents[t], slot, 1)
+    return out
+
+
 class SessionPool:
     """``sessions`` independent streaming sessions whose states stay on the GPU (``ng_pool_*``).
 
@@ -460,6 +472,73 @@ class SessionPool:
             raise ValueError(f'Need one token per session ({self.sessions})')
         self._check(self.lib.ng_pool_step(self.h, tokens, self.logits.ctypes.data, None, None))
         return self.logits.copy()
+
+    def reorder(self, beams, parents):
+        """Session w of each group of ``beams`` sessions takes over the state and logits of session
+        ``parents[group, w]`` of its group (parents [sessions // beams, beams], on the host)."""
+        parents = np.ascontiguousarray(parents, dtype=np.int32)
+        if beams < 1 or parents.shape != (self.sessions // beams, beams):
+            raise ValueError('Need one parent for each session, [sessions // beams, beams]')
+        self._check(self.lib.ng_pool_reorder(self.h, beams, parents.reshape(-1)))
+        rows = np.arange(self.sessions) // beams * beams + parents.reshape(-1)
+        self.logits = self.logits[rows]
+
+    def beam_search(self, prompts, beams, steps, end=None, allowed=None):
+        """Beam search over the pool's sessions, which form groups of ``beams``: each group continues
+        the session in its first slot.
+
+        ``prompts`` int [groups, time] (time >= 1) is fed to every beam, then ``steps`` tokens are
+        chosen.  Returns (tokens int32 [groups, beams, steps], scores float32 [groups, beams]),
+        best first: the cumulative log probability of the chosen tokens, over the tokens that
+        ``allowed`` (bool [264], default every byte and control token) admits.  A beam that has
+        chosen ``end`` is finished and continues with PAD at its score.  Afterwards each session has
+        been fed its own sequence, and ``logits`` holds its next logits.  The loop runs on the device
+        (token step, selection, reordering of states); tokens come back once, at the end.
+        """
+        from . import decoding
+        prompts = np.ascontiguousarray(prompts, dtype=np.int64)
+        if not 1 <= beams <= decoding.MAX_BEAMS or self.sessions % beams:
+            raise ValueError('Beams must be 1..32 and divide the pool\'s sessions')
+        groups = self.sessions // beams
+        if prompts.ndim != 2 or prompts.shape[0] != groups or prompts.shape[1] < 1:
+            raise ValueError(f'Need prompts [{groups}, time] with at least one token')
+        if ((prompts < 0) | (prompts >= VOCAB)).any():
+            raise ValueError('Token must be in 0..263')
+        if steps < 1:
+            raise ValueError('Need at least one step')
+        device = torch.device('cuda', self.lib.ng_pool_device(self.h))
+        # A stream of its own: the pool's calls take the default stream's handle, 0, for the engine's stream.
+        side = torch.cuda.Stream(device)
+        side.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.device(device), torch.cuda.stream(side):
+            stream = side.cuda_stream
+            logits = torch.empty((self.sessions, VOCAB), device=device)
+            feed = torch.from_numpy(prompts.T.astype(np.int32)).to(device).repeat_interleave(beams, 1)
+            if allowed is not None:
+                allowed = torch.as_tensor(allowed).to(device)
+            first = torch.zeros((groups, beams), dtype=torch.int32, device=device)
+            self._check(self.lib.ng_pool_reorder_device(self.h, beams, first.data_ptr(), stream))
+
+            def step(tokens):
+                self._check(self.lib.ng_pool_step_device(self.h, tokens.data_ptr(), logits.data_ptr(), stream))
+
+            for row in feed:
+                step(row)
+            scores = torch.full((groups, beams), -float('inf'), device=device)
+            scores[:, 0] = 0
+            finished = torch.zeros((groups, beams), dtype=torch.bool, device=device)
+            chosen = []
+            for _ in range(steps):
+                scores, tokens, parents, finished = decoding.beam_select(logits, scores, finished, allowed, end, PAD)
+                self._check(self.lib.ng_pool_reorder_device(self.h, beams, parents.data_ptr(), stream))
+                step(tokens)
+                chosen.append((tokens, parents))
+            tokens = torch.stack([t for t, _ in chosen]).cpu().numpy()
+            parents = torch.stack([p for _, p in chosen]).cpu().numpy()
+            scores = scores.cpu().numpy()
+            self.logits = logits.cpu().numpy()
+        self._check(self.lib.ng_pool_check(self.h))
+        return trace_beams(tokens, parents), scores
 
     def states(self):
         """Packed states [sessions, state_size] in the reference order."""
