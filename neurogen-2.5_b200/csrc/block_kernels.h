@@ -46,5 +46,8 @@ struct BlockMatmulArgs {
   int m, n, k;
 };
 void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s);
+// Throws when a product on this device reported a wait that ran out since the
+// last check (its result is lost; later products run normally).
+void check_block_matmul_errors(int device);
 
 } // namespace ngb

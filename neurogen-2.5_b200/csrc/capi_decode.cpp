@@ -133,6 +133,7 @@ int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale
     g.n = int(n);
     g.k = int(k);
     OnDevice on(device);
+    check_block_matmul_errors(device);
     launch_block_matmul(g, static_cast<cudaStream_t>(stream));
     NGB_CUDA(cudaGetLastError());
   });
