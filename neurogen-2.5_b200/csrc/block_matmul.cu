@@ -16,6 +16,7 @@
 #include <atomic>
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 
 namespace ngb {
 namespace {
@@ -112,69 +113,102 @@ __global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(BlockMatmulArgs a)
   }
 }
 
-// More rows: the tensor cores proper.  A tile is 128 weight rows (TMEM lanes)
-// x TN rows of a (TMEM columns).  One thread streams the blocks of 128 bytes
+// More rows: the tensor cores proper.  A tile is 128 rows of a (TMEM lanes) x
+// TN weight rows (TMEM columns).  One thread streams the blocks of 128 bytes
 // along k by TMA (SWIZZLE_128B, one swizzle atom a row), one issues each
 // block's four MMAs (M=128, N=TN, K=32) into a TMEM accumulator of its own (a
-// ring of them), and 4 or 8 warps add the finished accumulators, scaled, to
-// the sums in their registers: a thread holds one weight row, whose scale is
-// the tile's, and up to 128 columns, whose scales (times the weights') it
-// reads from shared memory four at a time.  Adding is a packed fma a pair.
+// ring of them), two warps stage the rows' scales, and 4 or 8 warps add the
+// finished accumulators, scaled, to the sums in their registers.  TN divides
+// 128 or is 256 in two halves, so a warp's columns share one weight scale and
+// a thread's row one scale of a: a block's addition is one packed fma a pair
+// of columns and nothing else.  The next 32 columns are on their way from
+// TMEM while the last ones are added.
 //
 // The CTAs either walk over the tiles (splits = 1), or, where the tiles are
 // too few to fill the GPU, `splits` CTAs of a cluster share a tile's k range:
-// each leaves its sums in shared memory and adds up a slice of the columns
-// over all of them, in rank order.
+// each leaves its sums in shared memory and adds up a slice of the rows over
+// all of them, in rank order.
 //
 // Every wait is bounded.  One that runs out sets *err; its role stops, waits
 // (bounded) for its own copies or MMAs in flight, and the CTA frees its TMEM.
-constexpr int kTileN = 128;       // weight rows of a tile
-constexpr int kScaleChunk = 32;   // blocks along k whose scales are staged at a time
+constexpr int kTileM = 128;       // rows of a in a tile
+constexpr int kScaleChunk = 16;   // blocks along k whose scales are staged at a time (two such buffers)
 constexpr long long kWaitClocks = 2000000000LL; // about a second
-constexpr uint32_t kTileWBytes = kTileN * kScaleBlock;
+constexpr uint32_t kTileABytes = kTileM * kScaleBlock;
 
 template <int TN> struct TcShape {
   static constexpr int kGroups = TN > 128 ? TN / 128 : 1; // of four epilogue warps
   static constexpr int kCols = TN / kGroups;              // columns a group adds up
-  // Two groups need more registers than 384 threads' even share: the groups
-  // raise their limit to kMoreRegs a thread, the four other warps (two of them
-  // idle) drop theirs; 256 * 208 + 128 * 80 <= 384 * 168 at launch.
-  static constexpr bool kShift = kGroups == 2;
-  static constexpr int kMoreRegs = 208, kFewerRegs = 80;
-  static constexpr int kEpilogue = 128 * kGroups, kThreads = kEpilogue + (kShift ? 128 : 64);
-  static constexpr uint32_t kStageBytes = kTileWBytes + TN * kScaleBlock;
+  // Epilogue warps, then one warp of copies, one of MMAs and two of scales.
+  static constexpr int kEpilogue = 128 * kGroups, kThreads = kEpilogue + 128;
+  static constexpr uint32_t kStageBytes = kTileABytes + TN * kScaleBlock;
   // More than half an SM's shared memory: one CTA an SM, so that a CTA never
   // waits for another's TMEM while its cluster waits for it.
-  static constexpr int kStages = TN == 256 ? 4 : TN == 128 ? 6 : 8;
+  static constexpr int kStages = TN == 256 ? 4 : TN == 128 ? 6 : 7;
   static constexpr int kAccs = TN == 256 ? 2 : 4, kTmemCols = kAccs * TN;
-  static constexpr int kScaleLd = TN + 4; // rows of 16 bytes, spread over the banks
-  static constexpr size_t kBars = 2 * kStages + 2 * kAccs + 1;
-  static constexpr size_t kSmem =
-      1024 + kStages * size_t(kStageBytes) + kScaleChunk * kScaleLd * 4 + kBars * 8 + 16;
-  static_assert(kSmem <= 232448, "shared memory");
-  static_assert(size_t(kTileN) * TN * 4 <= kStages * size_t(kStageBytes), "partial sums lie over the stages");
+  static constexpr int kPartLd = TN + 4; // row stride of a split's sums: 16-byte rows, spread over the banks
+  static constexpr size_t kBars = 2 * kStages + 2 * kAccs + 4 + 1;
+  static constexpr size_t kScaleFloats = 2 * kScaleChunk * (kTileM + kGroups);
+  static constexpr size_t kSwap = 4 * kGroups * 32 * 64; // 64 bytes of each row of a warp, on their way out
+  static constexpr size_t kSmem = 1024 + kStages * size_t(kStageBytes) + kSwap + kScaleFloats * 4 + kBars * 8 + 16;
+  static_assert(kSmem <= 232448 && kSmem > 116736, "shared memory");
+  static_assert(TN == 256 || size_t(kTileM) * kPartLd * 4 <= kStages * size_t(kStageBytes), "sums lie over the stages");
 };
+
+// Two groups need more registers than 384 threads' even share: they raise
+// their limit to kMoreRegs a thread and the four other warps drop theirs;
+// 256 * 216 + 128 * 72 <= 384 * 168 at launch.
+constexpr int kMoreRegs = 216, kFewerRegs = 72;
 
 // Instruction descriptor, kind::f8f6f4: D f32 (bits 4-5 = 1), A and B e4m3
 // (bits 7-9, 10-12 = 0), both K-major (bits 15, 16 = 0), N >> 3 at bits
 // 17-22, M >> 4 at bits 24-28.
-template <int TN> constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(TN >> 3) << 17) | (uint32_t(kTileN >> 4) << 24);
+template <int N> constexpr uint32_t kIdesc = (1u << 4) | (uint32_t(N >> 3) << 17) | (uint32_t(kTileM >> 4) << 24);
 
-template <int TN>
+template <int N>
 __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t accumulate) {
   asm volatile("{\n\t.reg .pred p;\n\t"
                "setp.ne.b32 p, %4, 0;\n\t"
                "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d_tmem), "l"(a), "l"(b), "r"(kIdesc<TN>), "r"(accumulate)
+               ::"r"(d_tmem), "l"(a), "l"(b), "r"(kIdesc<N>), "r"(accumulate)
                : "memory");
 }
 
-// sum += d * scale, two columns at a time.
-__device__ __forceinline__ void fma2(uint64_t &sum, float d0, float d1, float s0, float s1) {
-  uint64_t d, s;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(d0), "f"(d1));
-  asm("mov.b64 %0, {%1, %2};" : "=l"(s) : "f"(s0), "f"(s1));
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(d), "l"(s));
+// sum += d * scale, two columns at a time.  Volatile: kept behind the TMEM load
+// that was issued before it.
+__device__ __forceinline__ void fma2(uint64_t &sum, uint32_t d0, uint32_t d1, uint64_t scale) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(d), "l"(scale));
+}
+// 32 consecutive TMEM columns of this thread's lane: the load, and the wait
+// for every load issued, which the registers pass through so that no use of
+// them is moved before it.
+__device__ __forceinline__ void tmem_issue32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+               "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+               "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+                 "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+                 "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+                 "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+                 "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+               : "r"(addr));
+}
+__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
+                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
+                 "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+                 "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
+                 "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
+               ::"memory");
+  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+}
+__device__ __forceinline__ uint64_t pair(float v) {
+  uint64_t p;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(p) : "f"(v));
+  return p;
 }
 __device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
@@ -182,81 +216,192 @@ __device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) {
 
 __device__ __forceinline__ bool wait_bar(uint32_t bar, uint32_t parity, volatile int *abort_s) {
   if (mbar_try(bar, parity)) return true;
-  const long long t0 = clock64();
-  while (!mbar_try(bar, parity)) {
+  long long t0 = 0;
+#pragma unroll 1
+  for (int i = 1;; ++i) {
+    if (mbar_try(bar, parity)) return true;
+    if (i % 64) continue;
     if (*abort_s) return false;
-    if (clock64() - t0 > kWaitClocks) {
+    const long long t = clock64();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitClocks) {
       *abort_s = 1;
       return false;
     }
   }
-  return true;
+}
+// The same for a whole warp that goes on together or not at all.
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int *abort_s) {
+  return __all_sync(0xFFFFFFFFu, wait_bar(bar, parity, abort_s));
+}
+// True in one lane of the warp.
+__device__ __forceinline__ bool elect() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\t"
+               "elect.sync _|p, 0xFFFFFFFF;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(one));
+  return one != 0;
 }
 
-__device__ __forceinline__ void group_sync(int group) {
-  asm volatile("bar.sync %0, 128;" ::"r"(group + 1) : "memory");
+// Whether rows of the result, bias and memory term can be moved 16 bytes at a time.
+__host__ inline bool vector_rows(const BlockMatmulArgs &a) {
+  const auto ok = [](const void *p, long row_bytes) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row_bytes % 16 == 0;
+  };
+  return ok(a.y, a.ldy * long(elem_size(a.type))) && ok(a.bias, 0) && (!a.add || ok(a.add, a.ldadd * 4));
 }
 
-template <class Y> __device__ __forceinline__ Y from_f32(float v);
-template <> __device__ __forceinline__ float from_f32(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f32(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_f32(float v) { return __float2half_rn(v); }
+// Two values as 16-bit elements.
+template <class Y> __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t u;
+  if constexpr (std::is_same_v<Y, __nv_bfloat16>)
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(u) : "f"(hi), "f"(lo));
+  return u;
+}
 
-// One weight row's sums of kCols consecutive columns (rows m0.. of the result).
+template <class Y> __device__ __forceinline__ Y round_to(float v) {
+  if constexpr (std::is_same_v<Y, float>)
+    return v;
+  else if constexpr (std::is_same_v<Y, __nv_bfloat16>)
+    return __float2bfloat16_rn(v);
+  else
+    return __float2half_rn(v);
+}
+
+// A warp's 32 rows m0.. of kCols columns n0.., a row a lane in sum: bias and
+// memory term, rounding, store.  Where the columns are whole and aligned, each
+// 64 bytes of the rows change places in shared memory (16-byte pieces, spread
+// over the banks), so that a store instruction writes 8 rows x 64 bytes and
+// not 32 rows x 16.  The common path is kept short: it runs once a tile, from
+// instructions that the tile's main loop has pushed out of the cache.
 template <class Y, int kCols>
-__device__ __forceinline__ void store_sums(const BlockMatmulArgs &a, int m0, int n, const uint64_t (&sum)[kCols / 2]) {
-  if (n >= a.n) return;
-  const float bias = a.bias ? a.bias[n] : 0.f;
-  Y *y = static_cast<Y *>(a.y) + long(m0) * a.ldy + n;
-  const float *add = a.add ? a.add + long(m0) * a.ldadd + n : nullptr;
+__device__ __forceinline__ void store_rows(const BlockMatmulArgs &a, int m0, int n0, uint64_t (&sum)[kCols / 2],
+                                           bool vec, uint4 *swap) {
+  const int lane = threadIdx.x % 32, m = m0 + lane;
+  if (a.bias || a.add) {
+    const float *add = a.add + long(m) * a.ldadd + n0;
 #pragma unroll
-  for (int j = 0; j < kCols; j += 8) {
-    float v[8], e[8];
+    for (int j = 0; j < kCols; j += 2) {
+      float v[2];
+      unpack2(sum[j / 2], v[0], v[1]);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) unpack2(sum[(j + i) / 2], v[i], v[i + 1]);
-    if (add) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = m0 + j + i < a.m ? add[long(j + i) * a.ldadd] : 0.f;
+      for (int i = 0; i < 2; ++i) {
+        if (n0 + j + i >= a.n) continue;
+        if (a.bias) v[i] = __fadd_rn(v[i], a.bias[n0 + j + i]);
+        if (a.add && m < a.m) v[i] = __fmaf_rn(a.add_scale, add[j + i], v[i]);
+      }
+      asm("mov.b64 %0, {%1, %2};" : "=l"(sum[j / 2]) : "f"(v[0]), "f"(v[1]));
     }
+  }
+  Y *y = static_cast<Y *>(a.y);
+  if (vec && n0 + kCols <= a.n) {
+    constexpr int kStep = 64 / sizeof(Y); // columns in 64 bytes
+    const int piece = lane % 4, spread = lane / 2 % 4;
+    char *out = reinterpret_cast<char *>(y + long(m0 + lane / 4) * a.ldy + n0) + 16 * piece;
+    const long rows8 = 8 * a.ldy * long(sizeof(Y));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = __fadd_rn(v[i], bias);
-      if (add) v[i] = __fmaf_rn(a.add_scale, e[i], v[i]);
-      if (m0 + j + i < a.m) y[long(j + i) * a.ldy] = from_f32<Y>(v[i]);
+    for (int j = 0; j < kCols; j += kStep) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t u[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x, z;
+          if constexpr (sizeof(Y) == 2) {
+            unpack2(sum[j / 2 + 4 * i + e], x, z);
+            u[e] = pack16<Y>(x, z);
+          } else {
+            unpack2(sum[j / 2 + 2 * i + e / 2], x, z);
+            u[e] = __float_as_uint(e % 2 ? z : x);
+          }
+        }
+        swap[4 * lane + (i ^ spread)] = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + lane / 4;
+        const uint4 u = swap[4 * r + (piece ^ (r / 2 % 4))];
+        if (m0 + r < a.m) *reinterpret_cast<uint4 *>(out + i * rows8 + j * sizeof(Y)) = u;
+      }
+      __syncwarp();
+    }
+  } else if (m < a.m) {
+    y += long(m) * a.ldy + n0;
+#pragma unroll
+    for (int j = 0; j < kCols; j += 2) {
+      float x, z;
+      unpack2(sum[j / 2], x, z);
+      if (n0 + j < a.n) y[j] = round_to<Y>(x);
+      if (n0 + j + 1 < a.n) y[j + 1] = round_to<Y>(z);
     }
   }
 }
 
-template <int TN>
+// Four consecutive columns n.. of row m of a split's joined sums.
+template <class Y>
+__device__ __forceinline__ void store4(const BlockMatmulArgs &a, int m, int n, float4 s, bool vec) {
+  float v[4] = {s.x, s.y, s.z, s.w};
+  const bool whole = vec && n + 4 <= a.n;
+  if (whole) {
+    if (a.bias) {
+      const float4 b = *reinterpret_cast<const float4 *>(a.bias + n);
+      v[0] = __fadd_rn(v[0], b.x), v[1] = __fadd_rn(v[1], b.y), v[2] = __fadd_rn(v[2], b.z), v[3] = __fadd_rn(v[3], b.w);
+    }
+    if (a.add) {
+      const float4 e = *reinterpret_cast<const float4 *>(a.add + long(m) * a.ldadd + n);
+      const float c = a.add_scale;
+      v[0] = __fmaf_rn(c, e.x, v[0]), v[1] = __fmaf_rn(c, e.y, v[1]), v[2] = __fmaf_rn(c, e.z, v[2]), v[3] = __fmaf_rn(c, e.w, v[3]);
+    }
+    Y *y = static_cast<Y *>(a.y) + long(m) * a.ldy + n;
+    if constexpr (sizeof(Y) == 4)
+      *reinterpret_cast<float4 *>(y) = make_float4(v[0], v[1], v[2], v[3]);
+    else
+      *reinterpret_cast<uint2 *>(y) = make_uint2(pack16<Y>(v[0], v[1]), pack16<Y>(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < a.n) finish(a, m, n + i, v[i]);
+  }
+}
+
+template <int TN, class Y>
 __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
-    k_block_tc(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_a, BlockMatmulArgs a,
-               int splits, int tiles_n, int tiles, int *err, int stall_test) {
+    k_block_tc(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_w, BlockMatmulArgs a,
+               int splits, int tiles_n, int tiles, bool vec, int *err, int stall_test) {
   using S = TcShape<TN>;
   extern __shared__ uint8_t smem_raw[];
   // 128-byte swizzled tiles start on 1024-byte boundaries of the shared window.
-  uint8_t *stages = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u); // [kStages][weights, a]
-  float *scales = reinterpret_cast<float *>(stages + S::kStages * size_t(S::kStageBytes)); // [kScaleChunk][kScaleLd]
-  uint64_t *bars = reinterpret_cast<uint64_t *>(scales + kScaleChunk * S::kScaleLd);
+  uint8_t *stages = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u); // [kStages][a, weights]
+  uint4 *swap = reinterpret_cast<uint4 *>(stages + S::kStages * size_t(S::kStageBytes)); // [epilogue warps][32][4]
+  float *scales_a = reinterpret_cast<float *>(swap + S::kSwap / 16);                     // [2][kScaleChunk][kTileM]
+  float *scales_w = scales_a + 2 * kScaleChunk * kTileM;                                 // [2][kScaleChunk][kGroups]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(scales_w + 2 * kScaleChunk * S::kGroups);
   volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + S::kBars);
   volatile int *abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int kb = (a.k + kScaleBlock - 1) / kScaleBlock;
   const int z = blockIdx.x % splits, first = blockIdx.x / splits, stride = gridDim.x / splits;
   const int kb0 = int(long(z) * kb / splits), kb1 = int(long(z + 1) * kb / splits);
-  // full[stage], empty[stage]: a stage holds its block / has been read by its
-  // MMAs; ready[acc], taken[acc]: an accumulator holds its block's sum / has
-  // been added up.
+  // full / empty[stage]: a stage holds its block / has been read by its MMAs;
+  // ready / taken[acc]: an accumulator holds its block's sum / has been added
+  // up; sfull / sempty[buffer]: scales are staged / have been used.
   const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, ready = empty + 8 * S::kStages,
-                 taken = ready + 8 * S::kAccs, done = taken + 8 * S::kAccs;
+                 taken = ready + 8 * S::kAccs, sfull = taken + 8 * S::kAccs, sempty = sfull + 16, done = sempty + 16;
+  constexpr int kCopyWarp = S::kEpilogue / 32, kMmaWarp = kCopyWarp + 1, kScaleWarp = kCopyWarp + 2;
 
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
     for (int i = 0; i < S::kAccs; ++i) mbar_init(ready + 8 * i, 1), mbar_init(taken + 8 * i, 4 * S::kGroups);
+    for (int i = 0; i < 2; ++i) mbar_init(sfull + 8 * i, 2), mbar_init(sempty + 8 * i, 4 * S::kGroups);
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     *abort_s = stall_test; // test switch: the path of a wait that ran out, with nothing in flight
   }
-  if (warp == S::kEpilogue / 32 + 1) {
+  if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(const_cast<uint32_t *>(tmem_slot))),
                  "r"(S::kTmemCols)
@@ -269,113 +414,154 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   const bool stalled = *abort_s != 0;
 
-  uint64_t sum[S::kCols / 2];
-  const int group = warp / 4, row = tid % 128;
-  if (warp < S::kEpilogue / 32) {
-    if constexpr (S::kShift) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kMoreRegs));
+  if (warp < kCopyWarp) {
+    if constexpr (S::kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMoreRegs));
+    const int group = warp / 4, row = tid % 128;
+    const uint32_t from = tmem + (uint32_t(warp % 4 * 32) << 16) + group * S::kCols;
+    uint64_t sum[S::kCols / 2];
+    uint32_t d[2][32];
     bool alive = !stalled;
-    int it = 0; // accumulators taken so far
-    float *mine = scales + group * S::kCols;
-    for (int tile = first; tile < tiles; tile += stride) {
-      const int n0 = tile % tiles_n * kTileN, m0 = tile / tiles_n * TN + group * S::kCols;
+    int left = first < tiles ? ((tiles - 1 - first) / stride + 1) * (kb1 - kb0) : 0; // accumulators still to add
+    int acc = 0, chunk = 0; // accumulator in turn, scale buffers taken so far
+    uint32_t parity = 0;    // of the ring's round
+    // The first columns of the accumulator in turn, once it is ready, on their way to registers.
+    const auto begin = [&] {
+      alive = wait_warp(ready + 8 * acc, parity, abort_s);
+      fence_after();
+      if (alive) tmem_issue32(from + acc * TN, d[0]);
+    };
+    constexpr bool kAhead = S::kCols % 64 == 0; // an accumulator ends in d[1]: the next can begin in d[0]
+    if (kAhead && alive && left) begin();
+    for (int tile = first; tile < tiles && alive; tile += stride) {
 #pragma unroll
       for (int j = 0; j < S::kCols / 2; ++j) sum[j] = 0;
-      for (int c = kb0; c < kb1; c += kScaleChunk) {
-        // The scales of this chunk: lane = block along k, each warp a quarter of the columns.
-        group_sync(group); // the previous ones have been read
-        const int b = c + lane;
-        const float sw = b < kb1 ? a.w_scale[long(n0 / kScaleBlock) * kb + b] : 0.f;
-#pragma unroll 8
-        for (int j = warp % 4 * (S::kCols / 4); j < (warp % 4 + 1) * (S::kCols / 4); ++j)
-          mine[lane * S::kScaleLd + j] =
-              b < kb1 && m0 + j < a.m ? __fmul_rn(sw, a.a_scale[long(m0 + j) * kb + b]) : 0.f;
-        group_sync(group);
-        for (int b1 = c; b1 < min(c + kScaleChunk, kb1); ++b1, ++it) {
-          const int acc = it % S::kAccs;
-          if (alive) alive = __all_sync(0xFFFFFFFFu, wait_bar(ready + 8 * acc, (it / S::kAccs) & 1, abort_s));
-          if (!alive) continue; // the barriers above are still met
-          fence_after();
-          const uint32_t from = tmem + (uint32_t(warp % 4 * 32) << 16) + acc * TN + group * S::kCols;
-          const float4 *s4 = reinterpret_cast<const float4 *>(mine + (b1 - c) * S::kScaleLd);
+      for (int c = kb0; c < kb1 && alive; c += kScaleChunk, ++chunk) {
+        const int buf = chunk % 2;
+        alive = wait_warp(sfull + 8 * buf, (chunk / 2) & 1, abort_s);
+        const float *sa = scales_a + buf * kScaleChunk * kTileM + row, *sw = scales_w + buf * kScaleChunk * S::kGroups + group;
+        for (int b = min(kScaleChunk, kb1 - c); b > 0 && alive; --b, sa += kTileM, sw += S::kGroups) {
+          const uint64_t scale = pair(__fmul_rn(*sa, *sw));
+          if (!kAhead) begin();
+          if (!alive) break;
 #pragma unroll
           for (int j = 0; j < S::kCols; j += 32) {
-            float d[32];
-            tmem_ld32(from + j, d);
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 s = s4[(j + i) / 4];
-              fma2(sum[(j + i) / 2], d[i], d[i + 1], s.x, s.y);
-              fma2(sum[(j + i) / 2 + 1], d[i + 2], d[i + 3], s.z, s.w);
+            tmem_wait32(d[j / 32 % 2]);
+            if (j + 32 < S::kCols) {
+              tmem_issue32(from + acc * TN + j + 32, d[(j / 32 + 1) % 2]);
+            } else { // all of it is in registers
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(taken + 8 * acc);
+              acc = acc + 1 == S::kAccs ? 0 : acc + 1;
+              parity ^= acc == 0;
+              if (--left && kAhead) begin();
             }
-          }
-          fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(taken + 8 * acc);
-        }
-      }
-      if (splits == 1 && alive) {
-        if (a.type == Elem::f32)
-          store_sums<float, S::kCols>(a, m0, n0 + row, sum);
-        else if (a.type == Elem::bf16)
-          store_sums<__nv_bfloat16, S::kCols>(a, m0, n0 + row, sum);
-        else
-          store_sums<__half, S::kCols>(a, m0, n0 + row, sum);
-      }
-    }
-    if (splits > 1 && alive) {
-      // Every accumulator was ready, so every copy and MMA is done with the stages.
-      float *part = reinterpret_cast<float *>(stages) + group * S::kCols * kTileN;
 #pragma unroll
-      for (int j = 0; j < S::kCols; j += 2) {
-        float x, y;
-        unpack2(sum[j / 2], x, y);
-        part[j * kTileN + row] = x;
-        part[(j + 1) * kTileN + row] = y;
+            for (int i = 0; i < 32; i += 2) fma2(sum[(j + i) / 2], d[j / 32 % 2][i], d[j / 32 % 2][i + 1], scale);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sempty + 8 * buf);
+      }
+      if (!alive && left) break;
+      const int n0 = tile % tiles_n * TN + group * S::kCols, m0 = tile / tiles_n * kTileM + row / 32 * 32;
+      if (splits == 1) {
+        store_rows<Y, S::kCols>(a, m0, n0, sum, vec, swap + warp * 128);
+      } else {
+        // Every accumulator was ready, so every copy and MMA is done with the stages.
+        float *part = reinterpret_cast<float *>(stages) + row * S::kPartLd;
+#pragma unroll
+        for (int j = 0; j < S::kCols; j += 4) {
+          float4 v;
+          unpack2(sum[j / 2], v.x, v.y);
+          unpack2(sum[j / 2 + 1], v.z, v.w);
+          *reinterpret_cast<float4 *>(part + j) = v;
+        }
       }
     }
   } else {
-    if constexpr (S::kShift) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kFewerRegs));
-    if (warp == S::kEpilogue / 32 && lane == 0 && !stalled) { // copies
+    if constexpr (S::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewerRegs));
+    // The copies' and MMAs' warps run as one and elect the lane that issues:
+    // the instructions' operands stay in uniform registers.
+    if (warp == kCopyWarp && !stalled) {
       bool ok = true;
       int it = 0;
       for (int tile = first; tile < tiles && ok; tile += stride) {
-        const int n0 = tile % tiles_n * kTileN, m0 = tile / tiles_n * TN;
+        const int n0 = tile % tiles_n * TN, m0 = tile / tiles_n * kTileM;
         for (int b = kb0; b < kb1; ++b, ++it) {
           const int st = it % S::kStages;
-          if (it >= S::kStages) ok = wait_bar(empty + 8 * st, (it / S::kStages - 1) & 1, abort_s);
+          if (it >= S::kStages) ok = wait_warp(empty + 8 * st, (it / S::kStages - 1) & 1, abort_s);
           if (!ok) break;
-          const uint32_t dst = smem_u32(stages + st * size_t(S::kStageBytes));
-          mbar_expect(full + 8 * st, S::kStageBytes);
-          tma_load_2d(dst, &tm_w, b * kScaleBlock, n0, full + 8 * st);
-          tma_load_2d(dst + kTileWBytes, &tm_a, b * kScaleBlock, m0, full + 8 * st);
+          if (elect()) {
+            const uint32_t dst = smem_u32(stages + st * size_t(S::kStageBytes));
+            mbar_expect(full + 8 * st, S::kStageBytes);
+            tma_load_2d(dst, &tm_a, b * kScaleBlock, m0, full + 8 * st);
+            tma_load_2d(dst + kTileABytes, &tm_w, b * kScaleBlock, n0, full + 8 * st);
+          }
+          __syncwarp();
         }
       }
       // Copies in flight when a wait ran out, here or in another role.
       int none = 0;
       for (int i = max(0, it - S::kStages); i < it; ++i)
         wait_bar(full + 8 * (i % S::kStages), (i / S::kStages) & 1, &none);
-    }
-    if (warp == S::kEpilogue / 32 + 1 && lane == 0 && !stalled) { // MMAs
+    } else if (warp == kMmaWarp && !stalled) {
       bool ok = true;
       int it = 0;
+      const uint64_t desc_a = sw128_desc(smem_u32(stages)), desc_w = sw128_desc(smem_u32(stages) + kTileABytes);
       for (int tile = first; tile < tiles && ok; tile += stride) {
         for (int b = kb0; b < kb1; ++b, ++it) {
           const int st = it % S::kStages, acc = it % S::kAccs;
-          if (it >= S::kAccs) ok = wait_bar(taken + 8 * acc, (it / S::kAccs - 1) & 1, abort_s);
-          ok = ok && wait_bar(full + 8 * st, (it / S::kStages) & 1, abort_s);
+          ok = wait_warp(full + 8 * st, (it / S::kStages) & 1, abort_s);
+          if (ok && it >= S::kAccs) ok = wait_warp(taken + 8 * acc, (it / S::kAccs - 1) & 1, abort_s);
           if (!ok) break;
           fence_after();
-          const uint32_t w = smem_u32(stages + st * size_t(S::kStageBytes)), x = w + kTileWBytes;
+          if (elect()) {
+            const uint64_t at = uint64_t(st) * (S::kStageBytes >> 4); // descriptors count 16 bytes
 #pragma unroll
-          for (int j = 0; j < kScaleBlock / 32; ++j)
-            mma_f8<TN>(tmem + acc * TN, sw128_desc(w + 32 * j), sw128_desc(x + 32 * j), j > 0);
-          mma_commit(empty + 8 * st);
-          mma_commit(ready + 8 * acc);
+            for (int j = 0; j < kScaleBlock / 32; ++j)
+              mma_f8<TN>(tmem + acc * TN, desc_a + at + 2 * j, desc_w + at + 2 * j, j > 0);
+            mma_commit(empty + 8 * st);
+            mma_commit(ready + 8 * acc);
+          }
+          __syncwarp();
         }
       }
-      mma_commit(done); // arrives once every MMA above has completed
+      if (elect()) mma_commit(done); // arrives once every MMA above has completed
+      __syncwarp();
       int none = 0;
       wait_bar(done, 0, &none);
+    } else if (warp >= kScaleWarp && !stalled) {
+      // Lane = block along k and one of four rows; rows and blocks out of range count nothing.
+      const int quarter = (warp - kScaleWarp) * 2 + lane / kScaleChunk, at = lane % kScaleChunk;
+      bool ok = true;
+      int chunk = 0;
+      for (int tile = first; tile < tiles && ok; tile += stride) {
+        const int n0 = tile % tiles_n * TN, m0 = tile / tiles_n * kTileM;
+        for (int c = kb0; c < kb1; c += kScaleChunk, ++chunk) {
+          const int buf = chunk % 2, b = c + at;
+          if (chunk >= 2) ok = wait_warp(sempty + 8 * buf, (chunk / 2 - 1) & 1, abort_s);
+          if (!ok) break;
+          float *sa = scales_a + (buf * kScaleChunk + at) * kTileM;
+          const float *from = a.a_scale + long(m0 + quarter) * kb + b;
+#pragma unroll 1
+          for (int r = 0; r < kTileM; r += 64) {
+            float v[16]; // in flight together
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              v[i] = b < kb1 && m0 + quarter + r + 4 * i < a.m ? from[(r + 4 * i) * long(kb)] : 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sa[quarter + r + 4 * i] = v[i];
+          }
+          if (quarter < S::kGroups) {
+            const int n = n0 + quarter * S::kCols;
+            scales_w[(buf * kScaleChunk + at) * S::kGroups + quarter] =
+                b < kb1 && n < a.n ? a.w_scale[long(n / kScaleBlock) * kb + b] : 0.f;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sfull + 8 * buf);
+        }
+      }
     }
   }
   fence_before();
@@ -385,19 +571,23 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
   if (splits > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync(); // every CTA's sums are visible
-    if (!failed && tid < kTileN) {
-      const int tile = first, n = tile % tiles_n * kTileN + tid, m0 = tile / tiles_n * TN;
-      const float *part = reinterpret_cast<const float *>(stages);
-      const int j0 = z * TN / splits, j1 = (z + 1) * TN / splits;
-      for (int j = j0; j < j1; ++j) {
-        float v = 0.f;
-        for (int s = 0; s < splits; ++s) v = __fadd_rn(v, cluster.map_shared_rank(part, s)[j * kTileN + tid]);
-        if (n < a.n && m0 + j < a.m) finish(a, m0 + j, n, v);
+    if (!failed) {
+      const int n0 = first % tiles_n * TN, m0 = first / tiles_n * kTileM;
+      float *part = reinterpret_cast<float *>(stages);
+      const int r0 = z * kTileM / splits, r1 = min((z + 1) * kTileM / splits, a.m - m0);
+      for (int i = tid; i < (r1 - r0) * (TN / 4); i += S::kThreads) {
+        const int r = r0 + i / (TN / 4), j = i % (TN / 4) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < splits; ++s) {
+          const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(part, s) + r * S::kPartLd + j);
+          v.x = __fadd_rn(v.x, x.x), v.y = __fadd_rn(v.y, x.y), v.z = __fadd_rn(v.z, x.z), v.w = __fadd_rn(v.w, x.w);
+        }
+        store4<Y>(a, m0 + r, n0 + j, v, vec);
       }
     }
     cluster.sync(); // every CTA has read the others' sums
   }
-  if (warp == S::kEpilogue / 32 + 1) {
+  if (warp == kMmaWarp) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::kTmemCols) : "memory");
   }
@@ -425,10 +615,25 @@ struct DeviceSetup {
   std::atomic<int *> err{nullptr};
   int *err_dev = nullptr;
   int sms = 0;
+  int clusters[4] = {}; // clusters of 1, 2, 4 and 8 CTAs that run at once
 } g_setup[kMaxDevices];
 
+void cluster_config(cudaLaunchConfig_t &cfg, cudaLaunchAttribute *attr, int grid, int splits, int threads, size_t smem) {
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = splits > 1 ? 1 : 0;
+}
+
 template <int TN> void configure() {
-  NGB_CUDA(cudaFuncSetAttribute(k_block_tc<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(TcShape<TN>::kSmem)));
+  const int smem = int(TcShape<TN>::kSmem);
+  NGB_CUDA(cudaFuncSetAttribute(k_block_tc<TN, float>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  NGB_CUDA(cudaFuncSetAttribute(k_block_tc<TN, __nv_bfloat16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  NGB_CUDA(cudaFuncSetAttribute(k_block_tc<TN, __half>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
 }
 
 DeviceSetup &setup() {
@@ -444,6 +649,13 @@ DeviceSetup &setup() {
     cudaFuncAttributes fa;
     NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec)); // loads the kernel
     NGB_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device));
+    d.clusters[0] = d.sms;
+    for (int i = 1; i < 4; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[1];
+      cluster_config(cfg, attr, 1 << i, 1 << i, TcShape<128>::kThreads, TcShape<128>::kSmem);
+      NGB_CUDA(cudaOccupancyMaxActiveClusters(&d.clusters[i], k_block_tc<128, float>, &cfg));
+    }
     int *host = nullptr;
     NGB_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&host), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
     *host = 0;
@@ -467,22 +679,20 @@ int take_stall() {
 }
 
 template <int TN> void launch_tc(const BlockMatmulArgs &a, int splits, DeviceSetup &d, cudaStream_t s) {
-  CUtensorMap tm_w, tm_a;
-  if (!make_map(&tm_w, a.w, a.n, a.k, a.ldw, kTileN) || !make_map(&tm_a, a.a, a.m, a.k, a.lda, TN))
+  CUtensorMap tm_a, tm_w;
+  if (!make_map(&tm_a, a.a, a.m, a.k, a.lda, kTileM) || !make_map(&tm_w, a.w, a.n, a.k, a.ldw, TN))
     throw std::runtime_error("Cannot describe an 8-bit matrix to the copy engine");
-  const int tiles_n = (a.n + kTileN - 1) / kTileN, tiles = tiles_n * ((a.m + TN - 1) / TN);
+  const int tiles_n = (a.n + TN - 1) / TN, tiles = tiles_n * ((a.m + kTileM - 1) / kTileM);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(splits == 1 ? std::min(tiles, d.sms) : tiles * splits);
-  cfg.blockDim = dim3(TcShape<TN>::kThreads);
-  cfg.dynamicSmemBytes = TcShape<TN>::kSmem;
-  cfg.stream = s;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = splits;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = splits > 1 ? 1 : 0;
-  NGB_CUDA(cudaLaunchKernelEx(&cfg, k_block_tc<TN>, tm_w, tm_a, a, splits, tiles_n, tiles, d.err_dev, take_stall()));
+  cluster_config(cfg, attr, splits == 1 ? std::min(tiles, d.sms) : tiles * splits, splits, TcShape<TN>::kThreads,
+                 TcShape<TN>::kSmem);
+  cfg.stream = s;
+  const auto kernel = a.type == Elem::f32    ? k_block_tc<TN, float>
+                      : a.type == Elem::bf16 ? k_block_tc<TN, __nv_bfloat16>
+                                             : k_block_tc<TN, __half>;
+  NGB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_w, a, splits, tiles_n, tiles, vector_rows(a), d.err_dev,
+                              take_stall()));
 }
 
 // Tile width and k split: the shape with the least estimated time.  A CTA's
@@ -491,16 +701,17 @@ template <int TN> void launch_tc(const BlockMatmulArgs &a, int splits, DeviceSet
 struct Plan {
   int tn, splits;
 };
-Plan plan(const BlockMatmulArgs &a, int sms) {
-  const long kb = (a.k + kScaleBlock - 1) / kScaleBlock, tiles_n = (a.n + kTileN - 1) / kTileN;
+Plan plan(const BlockMatmulArgs &a, const DeviceSetup &d) {
+  const long kb = (a.k + kScaleBlock - 1) / kScaleBlock, tiles_m = (a.m + kTileM - 1) / kTileM;
   Plan best{128, 1};
   double least = 1e30;
   for (int tn : {32, 64, 128, 256}) {
-    const long tiles = tiles_n * ((a.m + tn - 1) / tn);
-    const double block = std::max(2.0 * tn, (kTileWBytes + tn * 128) / 80.0);
-    for (int splits : {1, 2, 4, 8}) {
-      if (splits > 1 && (splits > kb || tn > 128 || tiles * splits > sms)) continue;
-      const long waves = (tiles * splits + sms - 1) / sms;
+    const long tiles = tiles_m * ((a.n + tn - 1) / tn);
+    const double block = std::max(2.0 * tn, (kTileABytes + tn * 128) / 80.0);
+    for (int i = 0; i < 4; ++i) {
+      const int splits = 1 << i;
+      if (splits > 1 && (splits > kb || tn > 128 || tiles > d.clusters[i])) continue;
+      const long waves = (tiles + d.clusters[i] - 1) / d.clusters[i];
       const double t = 2500 + double(waves) * ((kb + splits - 1) / splits * block + 3.0 * tn) + (splits > 1 ? 1500 + 4.0 * tn : 0);
       if (t < least) least = t, best = {tn, splits};
     }
@@ -527,7 +738,7 @@ void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s) {
     k_block_vec<<<grid, 32 * kVecWarps, 0, s>>>(a);
     return;
   }
-  const Plan p = plan(a, d.sms);
+  const Plan p = plan(a, d);
   if (p.tn == 32)
     launch_tc<32>(a, p.splits, d, s);
   else if (p.tn == 64)
