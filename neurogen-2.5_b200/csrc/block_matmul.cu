@@ -63,52 +63,89 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Few rows of a (a single token's projection): bound by the weights' bytes.
-// CTA: 16 weight rows x 8 rows of a, the blocks along k dealt to 8 warps, whose
-// sums meet in shared memory in warp order.  Weights are the matrix
-// instruction's 16-row side.  A sum over k does not mind its order, so each
-// lane takes 16 consecutive bytes of its row (one load) and feeds them to two
-// instructions as if they were that instruction's own columns; both operands
-// are permuted alike.
+// Few rows of a (a single token's projection): bound by the weights' bytes, and
+// by latency where those are few.  CTA: 16 weight rows x 8 NT rows of a, the
+// blocks along k dealt to 8 warps, whose sums meet in shared memory in warp
+// order.  Weights are the matrix instruction's 16-row side.  A sum over k does
+// not mind its order, so each lane takes 16 consecutive bytes of its row (one
+// load) and feeds them to two instructions as if they were that instruction's
+// own columns; both operands are permuted alike.  A warp's loads of kAhead
+// blocks are in flight together.
 constexpr int kVecWarps = 8;
 
-__global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(BlockMatmulArgs a) {
-  __shared__ float part[kVecWarps][16 * 8];
+template <int NT> struct VecBlock {
+  static constexpr int kAhead = NT == 4 ? 2 : 4;
+  uint4 w[2][2], a[NT][2]; // [row or row + 8][half of the block], [8 rows of a][half]
+  float sw, sa[NT][2];
+};
+
+template <int NT> __global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(BlockMatmulArgs a, int tiles_n) {
+  __shared__ float part[kVecWarps][NT][8][16];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8;
+  const int n0 = blockIdx.x % tiles_n * 16, m0 = blockIdx.x / tiles_n * 8 * NT;
   const int kb = (a.k + kScaleBlock - 1) / kScaleBlock;
-  const int na = min(n0 + g, a.n - 1), nb = min(n0 + g + 8, a.n - 1), mg = m0 + g;
-  const uint8_t *wa = a.w + long(na) * a.ldw, *wb = a.w + long(nb) * a.ldw;
-  const uint8_t *ar = a.a + long(min(mg, a.m - 1)) * a.lda;
-  const int mc0 = min(m0 + 2 * t, a.m - 1), mc1 = min(m0 + 2 * t + 1, a.m - 1); // the result's columns of this lane
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int b = warp; b < kb; b += kVecWarps) {
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
+  const uint8_t *wa = a.w + long(min(n0 + g, a.n - 1)) * a.ldw, *wb = a.w + long(min(n0 + g + 8, a.n - 1)) * a.ldw;
+  const float *sw = a.w_scale + long(n0 / kScaleBlock) * kb;
+  const uint8_t *ar[NT];
+  const float *sa[NT][2]; // of the result's columns of this lane
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int k = b * kScaleBlock + h * 64 + t * 16;
-      const uint4 x = load16(wa, k, a.k), y = load16(wb, k, a.k), z = load16(ar, k, a.k);
-      mma_e4m3(d, x.x, y.x, x.y, y.y, z.x, z.y);
-      mma_e4m3(d, x.z, y.z, x.w, y.w, z.z, z.w);
-    }
-    const float sw = a.w_scale[long(n0 / kScaleBlock) * kb + b];
-    const float s0 = __fmul_rn(sw, a.a_scale[long(mc0) * kb + b]), s1 = __fmul_rn(sw, a.a_scale[long(mc1) * kb + b]);
-    sum[0] = __fmaf_rn(s0, d[0], sum[0]);
-    sum[1] = __fmaf_rn(s1, d[1], sum[1]);
-    sum[2] = __fmaf_rn(s0, d[2], sum[2]);
-    sum[3] = __fmaf_rn(s1, d[3], sum[3]);
+  for (int i = 0; i < NT; ++i) {
+    ar[i] = a.a + long(min(m0 + 8 * i + g, a.m - 1)) * a.lda;
+    sa[i][0] = a.a_scale + long(min(m0 + 8 * i + 2 * t, a.m - 1)) * kb;
+    sa[i][1] = a.a_scale + long(min(m0 + 8 * i + 2 * t + 1, a.m - 1)) * kb;
   }
-  float *mine = part[warp];
-  mine[(2 * t) * 16 + g] = sum[0];
-  mine[(2 * t + 1) * 16 + g] = sum[1];
-  mine[(2 * t) * 16 + g + 8] = sum[2];
-  mine[(2 * t + 1) * 16 + g + 8] = sum[3];
+  float sum[NT][4] = {};
+  for (int b0 = warp; b0 < kb; b0 += kVecWarps * VecBlock<NT>::kAhead) {
+    VecBlock<NT> v[VecBlock<NT>::kAhead];
+#pragma unroll
+    for (int u = 0; u < VecBlock<NT>::kAhead; ++u) {
+      const int b = b0 + u * kVecWarps;
+      if (b >= kb) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = b * kScaleBlock + h * 64 + t * 16;
+        v[u].w[0][h] = load16(wa, k, a.k);
+        v[u].w[1][h] = load16(wb, k, a.k);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) v[u].a[i][h] = load16(ar[i], k, a.k);
+      }
+      v[u].sw = sw[b];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) v[u].sa[i][0] = sa[i][0][b], v[u].sa[i][1] = sa[i][1][b];
+    }
+#pragma unroll
+    for (int u = 0; u < VecBlock<NT>::kAhead; ++u) {
+      if (b0 + u * kVecWarps >= kb) continue;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint4 x = v[u].w[0][h], y = v[u].w[1][h], z = v[u].a[i][h];
+          mma_e4m3(d, x.x, y.x, x.y, y.y, z.x, z.y);
+          mma_e4m3(d, x.z, y.z, x.w, y.w, z.z, z.w);
+        }
+        const float s0 = __fmul_rn(v[u].sw, v[u].sa[i][0]), s1 = __fmul_rn(v[u].sw, v[u].sa[i][1]);
+        sum[i][0] = __fmaf_rn(s0, d[0], sum[i][0]);
+        sum[i][1] = __fmaf_rn(s1, d[1], sum[i][1]);
+        sum[i][2] = __fmaf_rn(s0, d[2], sum[i][2]);
+        sum[i][3] = __fmaf_rn(s1, d[3], sum[i][3]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NT; ++i) {
+    part[warp][i][2 * t][g] = sum[i][0];
+    part[warp][i][2 * t + 1][g] = sum[i][1];
+    part[warp][i][2 * t][g + 8] = sum[i][2];
+    part[warp][i][2 * t + 1][g + 8] = sum[i][3];
+  }
   __syncthreads();
-  if (threadIdx.x < 128) {
-    const int n = n0 + threadIdx.x % 16, m = m0 + threadIdx.x / 16;
+  for (int e = threadIdx.x; e < 128 * NT; e += 32 * kVecWarps) {
+    const int n = n0 + e % 16, m = m0 + e / 16;
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < kVecWarps; ++i) v = __fadd_rn(v, part[i][threadIdx.x]);
+    for (int i = 0; i < kVecWarps; ++i) v = __fadd_rn(v, (&part[i][0][0][0])[e]);
     if (n < a.n && m < a.m) finish(a, m, n, v);
   }
 }
@@ -382,7 +419,8 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
   uint64_t *bars = reinterpret_cast<uint64_t *>(scales_w + 2 * kScaleChunk * S::kGroups);
   volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + S::kBars);
   volatile int *abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  // One value for the whole warp, known as such: the roles' branches are uniform.
+  const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0), lane = tid % 32;
   const int kb = (a.k + kScaleBlock - 1) / kScaleBlock;
   const int z = blockIdx.x % splits, first = blockIdx.x / splits, stride = gridDim.x / splits;
   const int kb0 = int(long(z) * kb / splits), kb1 = int(long(z + 1) * kb / splits);
@@ -647,7 +685,9 @@ DeviceSetup &setup() {
     configure<128>();
     configure<256>();
     cudaFuncAttributes fa;
-    NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec)); // loads the kernel
+    NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec<1>)); // loads the kernels
+    NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec<2>));
+    NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec<4>));
     NGB_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device));
     d.clusters[0] = d.sms;
     for (int i = 1; i < 4; ++i) {
@@ -676,6 +716,11 @@ int take_stall() {
   while (k > 0 && !left.compare_exchange_weak(k, k - 1)) {
   }
   return k > 0 ? 1 : 0;
+}
+
+template <int NT> void launch_vec(const BlockMatmulArgs &a, cudaStream_t s) {
+  const int tiles_n = (a.n + 15) / 16;
+  k_block_vec<NT><<<tiles_n * ((a.m + 8 * NT - 1) / (8 * NT)), 32 * kVecWarps, 0, s>>>(a, tiles_n);
 }
 
 template <int TN> void launch_tc(const BlockMatmulArgs &a, int splits, DeviceSetup &d, cudaStream_t s) {
@@ -734,8 +779,10 @@ void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s) {
   DeviceSetup &d = setup();
   // Few rows are bound by the weights' bytes, and by latency.
   if (a.m <= 16) {
-    const dim3 grid((a.n + 15) / 16, (a.m + 7) / 8);
-    k_block_vec<<<grid, 32 * kVecWarps, 0, s>>>(a);
+    if (a.m <= 8)
+      launch_vec<1>(a, s);
+    else
+      launch_vec<2>(a, s);
     return;
   }
   const Plan p = plan(a, d);
