@@ -163,12 +163,13 @@ template <int NT> __global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(
 //
 // The CTAs either walk over the tiles (splits = 1), or, where the tiles are
 // too few to fill the GPU, `splits` CTAs of a cluster share a tile's k range:
-// each leaves its sums in shared memory and adds up a slice of the rows over
-// all of them, in rank order.
+// each owns a slice of the rows, all send it their sums of these rows
+// (distributed shared memory), and it adds them up in rank order.
 //
 // Every wait is bounded.  One that runs out sets *err; its role stops, waits
 // (bounded) for its own copies or MMAs in flight, and the CTA frees its TMEM.
 constexpr int kTileM = 128;       // rows of a in a tile
+constexpr int kMaxSplits = 8;
 constexpr int kScaleChunk = 16;   // blocks along k whose scales are staged at a time (two such buffers)
 constexpr long long kWaitClocks = 2000000000LL; // about a second
 constexpr uint32_t kTileABytes = kTileM * kScaleBlock;
@@ -181,15 +182,16 @@ template <int TN> struct TcShape {
   static constexpr uint32_t kStageBytes = kTileABytes + TN * kScaleBlock;
   // More than half an SM's shared memory: one CTA an SM, so that a CTA never
   // waits for another's TMEM while its cluster waits for it.
-  static constexpr int kStages = TN == 256 ? 4 : TN == 128 ? 6 : 7;
+  static constexpr int kStages = TN == 256 || TN == 128 ? 4 : 6;
   static constexpr int kAccs = TN == 256 ? 2 : 4, kTmemCols = kAccs * TN;
-  static constexpr int kPartLd = TN + 4; // row stride of a split's sums: 16-byte rows, spread over the banks
   static constexpr size_t kBars = 2 * kStages + 2 * kAccs + 4 + 1;
   static constexpr size_t kScaleFloats = 2 * kScaleChunk * (kTileM + kGroups);
   static constexpr size_t kSwap = 4 * kGroups * 32 * 64; // 64 bytes of each row of a warp, on their way out
-  static constexpr size_t kSmem = 1024 + kStages * size_t(kStageBytes) + kSwap + kScaleFloats * 4 + kBars * 8 + 16;
+  // A split's sums of the rows a CTA owns: [splits][TN / 4][rows + 1] of 16 bytes.
+  static constexpr size_t kPart = TN == 256 ? 0 : TN * 4 * size_t(kTileM + kMaxSplits);
+  static constexpr size_t kSmem =
+      1024 + kStages * size_t(kStageBytes) + kPart + kSwap + kScaleFloats * 4 + kBars * 8 + 16;
   static_assert(kSmem <= 232448 && kSmem > 116736, "shared memory");
-  static_assert(TN == 256 || size_t(kTileM) * kPartLd * 4 <= kStages * size_t(kStageBytes), "sums lie over the stages");
 };
 
 // Two groups need more registers than 384 threads' even share: they raise
@@ -280,6 +282,10 @@ __device__ __forceinline__ bool elect() {
                : "=r"(one));
   return one != 0;
 }
+
+// Every CTA of the cluster has come here; what it wrote before is visible.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // Whether rows of the result, bias and memory term can be moved 16 bytes at a time.
 __host__ inline bool vector_rows(const BlockMatmulArgs &a) {
@@ -413,9 +419,10 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   // 128-byte swizzled tiles start on 1024-byte boundaries of the shared window.
   uint8_t *stages = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u); // [kStages][a, weights]
-  uint4 *swap = reinterpret_cast<uint4 *>(stages + S::kStages * size_t(S::kStageBytes)); // [epilogue warps][32][4]
-  float *scales_a = reinterpret_cast<float *>(swap + S::kSwap / 16);                     // [2][kScaleChunk][kTileM]
-  float *scales_w = scales_a + 2 * kScaleChunk * kTileM;                                 // [2][kScaleChunk][kGroups]
+  float4 *part = reinterpret_cast<float4 *>(stages + S::kStages * size_t(S::kStageBytes));
+  uint4 *swap = reinterpret_cast<uint4 *>(part + S::kPart / 16);     // [epilogue warps][32][4]
+  float *scales_a = reinterpret_cast<float *>(swap + S::kSwap / 16); // [2][kScaleChunk][kTileM]
+  float *scales_w = scales_a + 2 * kScaleChunk * kTileM;             // [2][kScaleChunk][kGroups]
   uint64_t *bars = reinterpret_cast<uint64_t *>(scales_w + 2 * kScaleChunk * S::kGroups);
   volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + S::kBars);
   volatile int *abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -431,26 +438,54 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
                  taken = ready + 8 * S::kAccs, sfull = taken + 8 * S::kAccs, sempty = sfull + 16, done = sempty + 16;
   constexpr int kCopyWarp = S::kEpilogue / 32, kMmaWarp = kCopyWarp + 1, kScaleWarp = kCopyWarp + 2;
 
-  if (tid == 0) {
-    for (int i = 0; i < S::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
-    for (int i = 0; i < S::kAccs; ++i) mbar_init(ready + 8 * i, 1), mbar_init(taken + 8 * i, 4 * S::kGroups);
-    for (int i = 0; i < 2; ++i) mbar_init(sfull + 8 * i, 2), mbar_init(sempty + 8 * i, 4 * S::kGroups);
-    mbar_init(done, 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    *abort_s = stall_test; // test switch: the path of a wait that ran out, with nothing in flight
-  }
-  if (warp == kMmaWarp) {
+  const bool stalled = stall_test != 0; // test switch: the path of a wait that ran out, with nothing in flight
+  const auto copy_block = [&](int st, int b, int tile) {
+    const uint32_t dst = smem_u32(stages + st * size_t(S::kStageBytes));
+    mbar_expect(full + 8 * st, S::kStageBytes);
+    tma_load_2d(dst, &tm_a, b * kScaleBlock, tile / tiles_n * kTileM, full + 8 * st);
+    tma_load_2d(dst + kTileABytes, &tm_w, b * kScaleBlock, tile % tiles_n * TN, full + 8 * st);
+  };
+  // Scales of 16 blocks along k from b on: lane = block and one of four rows
+  // (two warps), rows and blocks out of range count nothing.
+  const int quarter = (warp - kScaleWarp) * 2 + lane / kScaleChunk, at = lane % kScaleChunk;
+  constexpr int kBatch = S::kGroups == 1 ? 32 : 16; // loads in flight together
+  float v[kBatch], vw;
+  const auto load_scales = [&](int tile, int c, int r) {
+    const int b = c + at, m = tile / tiles_n * kTileM + quarter + r, n = tile % tiles_n * TN + quarter * S::kCols;
+    const float *from = a.a_scale + long(m) * kb + b;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) v[i] = b < kb1 && m + 4 * i < a.m ? from[4 * i * long(kb)] : 0.f;
+    vw = quarter < S::kGroups && b < kb1 && n < a.n ? a.w_scale[long(n / kScaleBlock) * kb + b] : 0.f;
+  };
+  // Before the CTA meets, only what does not make it wait.
+  if (warp == kCopyWarp) {
+    if (lane == 0) {
+      for (int i = 0; i < S::kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+      for (int i = 0; i < S::kAccs; ++i) mbar_init(ready + 8 * i, 1), mbar_init(taken + 8 * i, 4 * S::kGroups);
+      for (int i = 0; i < 2; ++i) mbar_init(sfull + 8 * i, 2), mbar_init(sempty + 8 * i, 4 * S::kGroups);
+      mbar_init(done, 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      *abort_s = stall_test;
+    }
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_a)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tm_w)) : "memory");
+    }
+    __syncwarp();
+  } else if (warp >= kScaleWarp) {
+    if (first < tiles) load_scales(first, kb0, 0);
+  } else if (warp == kMmaWarp) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(const_cast<uint32_t *>(tmem_slot))),
                  "r"(S::kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (splits > 1) cluster_arrive(); // this CTA runs: the others may write to its shared memory
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;
-  const bool stalled = *abort_s != 0;
 
   if (warp < kCopyWarp) {
     if constexpr (S::kGroups == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kMoreRegs));
@@ -506,17 +541,19 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
       if (splits == 1) {
         store_rows<Y, S::kCols>(a, m0, n0, sum, vec, swap + warp * 128);
       } else {
-        // Every accumulator was ready, so every copy and MMA is done with the stages.
-        float *part = reinterpret_cast<float *>(stages) + row * S::kPartLd;
+        cluster_wait();
+        const int rows = kTileM / splits, owner = row / rows;
+        float4 *to = cg::this_cluster().map_shared_rank(part, owner) + long(z) * (S::kCols / 4) * (rows + 1) + row % rows;
 #pragma unroll
         for (int j = 0; j < S::kCols; j += 4) {
           float4 v;
           unpack2(sum[j / 2], v.x, v.y);
           unpack2(sum[j / 2 + 1], v.z, v.w);
-          *reinterpret_cast<float4 *>(part + j) = v;
+          to[j / 4 * (rows + 1)] = v;
         }
       }
     }
+    if (splits > 1 && !alive) cluster_wait();
   } else {
     if constexpr (S::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewerRegs));
     // The copies' and MMAs' warps run as one and elect the lane that issues:
@@ -525,17 +562,11 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
       bool ok = true;
       int it = 0;
       for (int tile = first; tile < tiles && ok; tile += stride) {
-        const int n0 = tile % tiles_n * TN, m0 = tile / tiles_n * kTileM;
         for (int b = kb0; b < kb1; ++b, ++it) {
           const int st = it % S::kStages;
           if (it >= S::kStages) ok = wait_warp(empty + 8 * st, (it / S::kStages - 1) & 1, abort_s);
           if (!ok) break;
-          if (elect()) {
-            const uint32_t dst = smem_u32(stages + st * size_t(S::kStageBytes));
-            mbar_expect(full + 8 * st, S::kStageBytes);
-            tma_load_2d(dst, &tm_a, b * kScaleBlock, m0, full + 8 * st);
-            tma_load_2d(dst + kTileABytes, &tm_w, b * kScaleBlock, n0, full + 8 * st);
-          }
+          if (elect()) copy_block(st, b, tile);
           __syncwarp();
         }
       }
@@ -570,60 +601,57 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
       int none = 0;
       wait_bar(done, 0, &none);
     } else if (warp >= kScaleWarp && !stalled) {
-      // Lane = block along k and one of four rows; rows and blocks out of range count nothing.
-      const int quarter = (warp - kScaleWarp) * 2 + lane / kScaleChunk, at = lane % kScaleChunk;
       bool ok = true;
       int chunk = 0;
       for (int tile = first; tile < tiles && ok; tile += stride) {
-        const int n0 = tile % tiles_n * TN, m0 = tile / tiles_n * kTileM;
         for (int c = kb0; c < kb1; c += kScaleChunk, ++chunk) {
-          const int buf = chunk % 2, b = c + at;
+          const int buf = chunk % 2;
           if (chunk >= 2) ok = wait_warp(sempty + 8 * buf, (chunk / 2 - 1) & 1, abort_s);
           if (!ok) break;
           float *sa = scales_a + (buf * kScaleChunk + at) * kTileM;
-          const float *from = a.a_scale + long(m0 + quarter) * kb + b;
 #pragma unroll 1
-          for (int r = 0; r < kTileM; r += 64) {
-            float v[16]; // in flight together
+          for (int r = 0; r < kTileM; r += 4 * kBatch) {
+            if (r > 0) load_scales(tile, c, r);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              v[i] = b < kb1 && m0 + quarter + r + 4 * i < a.m ? from[(r + 4 * i) * long(kb)] : 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sa[quarter + r + 4 * i] = v[i];
+            for (int i = 0; i < kBatch; ++i) sa[quarter + r + 4 * i] = v[i];
           }
-          if (quarter < S::kGroups) {
-            const int n = n0 + quarter * S::kCols;
-            scales_w[(buf * kScaleChunk + at) * S::kGroups + quarter] =
-                b < kb1 && n < a.n ? a.w_scale[long(n / kScaleBlock) * kb + b] : 0.f;
-          }
+          if (quarter < S::kGroups) scales_w[(buf * kScaleChunk + at) * S::kGroups + quarter] = vw;
           __syncwarp();
           if (lane == 0) mbar_arrive(sfull + 8 * buf);
+          // The next ones, while these are used.
+          if (c + kScaleChunk < kb1)
+            load_scales(tile, c + kScaleChunk, 0);
+          else if (tile + stride < tiles)
+            load_scales(tile + stride, kb0, 0);
         }
       }
     }
+    if (splits > 1) cluster_wait();
   }
   fence_before();
   __syncthreads();
   const bool failed = *abort_s != 0;
   if (failed && tid == 0) *reinterpret_cast<volatile int *>(err) = 1;
   if (splits > 1) {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync(); // every CTA's sums are visible
+    cluster_arrive();
+    cluster_wait(); // every CTA has sent its sums
     if (!failed) {
-      const int n0 = first % tiles_n * TN, m0 = first / tiles_n * kTileM;
-      float *part = reinterpret_cast<float *>(stages);
-      const int r0 = z * kTileM / splits, r1 = min((z + 1) * kTileM / splits, a.m - m0);
-      for (int i = tid; i < (r1 - r0) * (TN / 4); i += S::kThreads) {
-        const int r = r0 + i / (TN / 4), j = i % (TN / 4) * 4;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < splits; ++s) {
-          const float4 x = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(part, s) + r * S::kPartLd + j);
-          v.x = __fadd_rn(v.x, x.x), v.y = __fadd_rn(v.y, x.y), v.z = __fadd_rn(v.z, x.z), v.w = __fadd_rn(v.w, x.w);
-        }
-        store4<Y>(a, m0 + r, n0 + j, v, vec);
+      const int n0 = first % tiles_n * TN, rows = kTileM / splits, m0 = first / tiles_n * kTileM + z * rows;
+      const int valid = min(rows, a.m - m0);
+      for (int i = tid; i < valid * (TN / 4); i += S::kThreads) {
+        const int r = i / (TN / 4), j = i % (TN / 4);
+        float4 x[kMaxSplits];
+#pragma unroll
+        for (int s = 0; s < kMaxSplits; ++s)
+          if (s < splits) x[s] = part[(long(s) * (TN / 4) + j) * (rows + 1) + r];
+        float4 v = x[0];
+#pragma unroll
+        for (int s = 1; s < kMaxSplits; ++s)
+          if (s < splits)
+            v.x = __fadd_rn(v.x, x[s].x), v.y = __fadd_rn(v.y, x[s].y), v.z = __fadd_rn(v.z, x[s].z), v.w = __fadd_rn(v.w, x[s].w);
+        store4<Y>(a, m0 + r, n0 + 4 * j, v, vec);
       }
     }
-    cluster.sync(); // every CTA has read the others' sums
   }
   if (warp == kMmaWarp) {
     fence_after();
