@@ -14,6 +14,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <climits>
+#include <cmath>
 #include <cstdlib>
 #include <mutex>
 #include <type_traits>
@@ -69,17 +71,17 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
 // order.  Weights are the matrix instruction's 16-row side.  A sum over k does
 // not mind its order, so each lane takes 16 consecutive bytes of its row (one
 // load) and feeds them to two instructions as if they were that instruction's
-// own columns; both operands are permuted alike.  A warp's loads of kAhead
-// blocks are in flight together.
+// own columns; both operands are permuted alike.  A warp's loads of AHEAD
+// blocks are in flight together, and CTAS CTAs share an SM.
 constexpr int kVecWarps = 8;
 
 template <int NT> struct VecBlock {
-  static constexpr int kAhead = NT == 4 ? 2 : 4;
   uint4 w[2][2], a[NT][2]; // [row or row + 8][half of the block], [8 rows of a][half]
   float sw, sa[NT][2];
 };
 
-template <int NT> __global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(BlockMatmulArgs a, int tiles_n) {
+template <int NT, int AHEAD, int CTAS>
+__global__ void __launch_bounds__(32 * kVecWarps, CTAS) k_block_vec(BlockMatmulArgs a, int tiles_n) {
   __shared__ float part[kVecWarps][NT][8][16];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, t = lane % 4;
   const int n0 = blockIdx.x % tiles_n * 16, m0 = blockIdx.x / tiles_n * 8 * NT;
@@ -95,10 +97,10 @@ template <int NT> __global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(
     sa[i][1] = a.a_scale + long(min(m0 + 8 * i + 2 * t + 1, a.m - 1)) * kb;
   }
   float sum[NT][4] = {};
-  for (int b0 = warp; b0 < kb; b0 += kVecWarps * VecBlock<NT>::kAhead) {
-    VecBlock<NT> v[VecBlock<NT>::kAhead];
+  for (int b0 = warp; b0 < kb; b0 += kVecWarps * AHEAD) {
+    VecBlock<NT> v[AHEAD];
 #pragma unroll
-    for (int u = 0; u < VecBlock<NT>::kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       const int b = b0 + u * kVecWarps;
       if (b >= kb) continue;
 #pragma unroll
@@ -114,7 +116,7 @@ template <int NT> __global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(
       for (int i = 0; i < NT; ++i) v[u].sa[i][0] = sa[i][0][b], v[u].sa[i][1] = sa[i][1][b];
     }
 #pragma unroll
-    for (int u = 0; u < VecBlock<NT>::kAhead; ++u) {
+    for (int u = 0; u < AHEAD; ++u) {
       if (b0 + u * kVecWarps >= kb) continue;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -153,13 +155,16 @@ template <int NT> __global__ void __launch_bounds__(32 * kVecWarps) k_block_vec(
 // More rows: the tensor cores proper.  A tile is 128 rows of a (TMEM lanes) x
 // TN weight rows (TMEM columns).  One thread streams the blocks of 128 bytes
 // along k by TMA (SWIZZLE_128B, one swizzle atom a row), one issues each
-// block's four MMAs (M=128, N=TN, K=32) into a TMEM accumulator of its own (a
-// ring of them), two warps stage the rows' scales, and 4 or 8 warps add the
+// block's four MMAs (M=128, N=TN, K=32) into a TMEM accumulator of its own, two warps stage the rows' scales, and 4 or 8 warps add the
 // finished accumulators, scaled, to the sums in their registers.  TN divides
 // 128 or is 256 in two halves, so a warp's columns share one weight scale and
 // a thread's row one scale of a: a block's addition is one packed fma a pair
 // of columns and nothing else.  The next 32 columns are on their way from
 // TMEM while the last ones are added.
+//
+// The roles meet (mbarriers) once for kPair blocks: a meeting costs the MMAs'
+// thread some 400 clocks, more than a block's MMAs take when TN is small
+// (512 x 768 x 3200, TN = 32: one block a meeting 10.8 us, two 9.2 us).
 //
 // The CTAs either walk over the tiles (splits = 1), or, where the tiles are
 // too few to fill the GPU, `splits` CTAs of a cluster share a tile's k range:
@@ -179,16 +184,18 @@ template <int TN> struct TcShape {
   static constexpr int kCols = TN / kGroups;              // columns a group adds up
   // Epilogue warps, then one warp of copies, one of MMAs and two of scales.
   static constexpr int kEpilogue = 128 * kGroups, kThreads = kEpilogue + 128;
-  static constexpr uint32_t kStageBytes = kTileABytes + TN * kScaleBlock;
+  static constexpr int kPair = TN == 256 ? 1 : 2; // blocks a stage and a set of accumulators hold
+  static constexpr uint32_t kBlockBytes = kTileABytes + TN * kScaleBlock, kStageBytes = kPair * kBlockBytes;
   // More than half an SM's shared memory: one CTA an SM, so that a CTA never
   // waits for another's TMEM while its cluster waits for it.
-  static constexpr int kStages = TN == 256 || TN == 128 ? 4 : 6;
-  static constexpr int kAccs = TN == 256 ? 2 : 4, kTmemCols = kAccs * TN;
+  static constexpr int kStages = TN == 256 ? 4 : 3;
+  static constexpr int kAccs = TN == 32 ? 4 : 2, kTmemCols = kAccs * kPair * TN; // sets of accumulators
   static constexpr size_t kBars = 2 * kStages + 2 * kAccs + 4 + 1;
   static constexpr size_t kScaleFloats = 2 * kScaleChunk * (kTileM + kGroups);
   static constexpr size_t kSwap = 4 * kGroups * 32 * 64; // 64 bytes of each row of a warp, on their way out
-  // A split's sums of the rows a CTA owns: [splits][TN / 4][rows + 1] of 16 bytes.
-  static constexpr size_t kPart = TN == 256 ? 0 : TN * 4 * size_t(kTileM + kMaxSplits);
+  // A split's sums of the rows a CTA owns: [splits][TN / 4][rows + 1] of 16
+  // bytes (narrow tiles only: with 128 columns or more there are no splits).
+  static constexpr size_t kPart = TN >= 128 ? 0 : TN * 4 * size_t(kTileM + kMaxSplits);
   static constexpr size_t kSmem =
       1024 + kStages * size_t(kStageBytes) + kPart + kSwap + kScaleFloats * 4 + kBars * 8 + 16;
   static_assert(kSmem <= 232448 && kSmem > 116736, "shared memory");
@@ -305,21 +312,13 @@ template <class Y> __device__ __forceinline__ uint32_t pack16(float lo, float hi
   return u;
 }
 
-template <class Y> __device__ __forceinline__ Y round_to(float v) {
-  if constexpr (std::is_same_v<Y, float>)
-    return v;
-  else if constexpr (std::is_same_v<Y, __nv_bfloat16>)
-    return __float2bfloat16_rn(v);
-  else
-    return __float2half_rn(v);
-}
-
 // A warp's 32 rows m0.. of kCols columns n0.., a row a lane in sum: bias and
-// memory term, rounding, store.  Where the columns are whole and aligned, each
-// 64 bytes of the rows change places in shared memory (16-byte pieces, spread
-// over the banks), so that a store instruction writes 8 rows x 64 bytes and
-// not 32 rows x 16.  The common path is kept short: it runs once a tile, from
-// instructions that the tile's main loop has pushed out of the cache.
+// memory term, rounding, store.  Each 64 bytes of the rows change places in
+// shared memory (16-byte pieces, spread over the banks), so that a store
+// instruction writes 8 rows x 64 bytes and not 32 rows x 16; where the rows
+// are not aligned for that, 32 elements of them.  The code is kept short: it
+// runs once a tile, from instructions that the tile's main loop has pushed out
+// of the cache.
 template <class Y, int kCols>
 __device__ __forceinline__ void store_rows(const BlockMatmulArgs &a, int m0, int n0, uint64_t (&sum)[kCols / 2],
                                            bool vec, uint4 *swap) {
@@ -339,48 +338,47 @@ __device__ __forceinline__ void store_rows(const BlockMatmulArgs &a, int m0, int
       asm("mov.b64 %0, {%1, %2};" : "=l"(sum[j / 2]) : "f"(v[0]), "f"(v[1]));
     }
   }
-  Y *y = static_cast<Y *>(a.y);
-  if (vec && n0 + kCols <= a.n) {
-    constexpr int kStep = 64 / sizeof(Y); // columns in 64 bytes
-    const int piece = lane % 4, spread = lane / 2 % 4;
-    char *out = reinterpret_cast<char *>(y + long(m0 + lane / 4) * a.ldy + n0) + 16 * piece;
-    const long rows8 = 8 * a.ldy * long(sizeof(Y));
+  constexpr int kStep = 64 / sizeof(Y), kPiece = 16 / sizeof(Y); // columns in 64 bytes, in 16
+  const int piece = lane % 4, spread = lane / 2 % 4;
+  Y *y = static_cast<Y *>(a.y) + long(m0) * a.ldy + n0;
+  const bool whole = vec && a.n % kPiece == 0;
 #pragma unroll
-    for (int j = 0; j < kCols; j += kStep) {
+  for (int j = 0; j < kCols; j += kStep) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t u[4];
+    for (int i = 0; i < 4; ++i) {
+      uint32_t u[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float x, z;
-          if constexpr (sizeof(Y) == 2) {
-            unpack2(sum[j / 2 + 4 * i + e], x, z);
-            u[e] = pack16<Y>(x, z);
-          } else {
-            unpack2(sum[j / 2 + 2 * i + e / 2], x, z);
-            u[e] = __float_as_uint(e % 2 ? z : x);
-          }
+      for (int e = 0; e < 4; ++e) {
+        float x, z;
+        if constexpr (sizeof(Y) == 2) {
+          unpack2(sum[j / 2 + 4 * i + e], x, z);
+          u[e] = pack16<Y>(x, z);
+        } else {
+          unpack2(sum[j / 2 + 2 * i + e / 2], x, z);
+          u[e] = __float_as_uint(e % 2 ? z : x);
         }
-        swap[4 * lane + (i ^ spread)] = make_uint4(u[0], u[1], u[2], u[3]);
       }
-      __syncwarp();
+      swap[4 * lane + (i ^ spread)] = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    __syncwarp();
+    if (whole) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 8 * i + lane / 4;
         const uint4 u = swap[4 * r + (piece ^ (r / 2 % 4))];
-        if (m0 + r < a.m) *reinterpret_cast<uint4 *>(out + i * rows8 + j * sizeof(Y)) = u;
+        if (m0 + r < a.m && n0 + j + piece * kPiece < a.n)
+          *reinterpret_cast<uint4 *>(y + r * a.ldy + j + piece * kPiece) = u;
       }
-      __syncwarp();
+    } else {
+      const Y *held = reinterpret_cast<const Y *>(swap);
+#pragma unroll 4
+      for (int i = 0; i < kStep; ++i) { // 32 elements an iteration, along the rows
+        const int r = (32 * i + lane) / kStep, col = (32 * i + lane) % kStep;
+        const Y v = held[(4 * r + ((col / kPiece) ^ (r / 2 % 4))) * kPiece + col % kPiece];
+        if (m0 + r < a.m && n0 + j + col < a.n) y[r * a.ldy + j + col] = v;
+      }
     }
-  } else if (m < a.m) {
-    y += long(m) * a.ldy + n0;
-#pragma unroll
-    for (int j = 0; j < kCols; j += 2) {
-      float x, z;
-      unpack2(sum[j / 2], x, z);
-      if (n0 + j < a.n) y[j] = round_to<Y>(x);
-      if (n0 + j + 1 < a.n) y[j + 1] = round_to<Y>(z);
-    }
+    __syncwarp();
   }
 }
 
@@ -431,20 +429,14 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
   const int kb = (a.k + kScaleBlock - 1) / kScaleBlock;
   const int z = blockIdx.x % splits, first = blockIdx.x / splits, stride = gridDim.x / splits;
   const int kb0 = int(long(z) * kb / splits), kb1 = int(long(z + 1) * kb / splits);
-  // full / empty[stage]: a stage holds its block / has been read by its MMAs;
-  // ready / taken[acc]: an accumulator holds its block's sum / has been added
-  // up; sfull / sempty[buffer]: scales are staged / have been used.
+  // full / empty[stage]: a stage holds its blocks / has been read by its MMAs;
+  // ready / taken[acc]: a set of accumulators holds its blocks' sums / has been
+  // added up; sfull / sempty[buffer]: scales are staged / have been used.
   const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, ready = empty + 8 * S::kStages,
                  taken = ready + 8 * S::kAccs, sfull = taken + 8 * S::kAccs, sempty = sfull + 16, done = sempty + 16;
   constexpr int kCopyWarp = S::kEpilogue / 32, kMmaWarp = kCopyWarp + 1, kScaleWarp = kCopyWarp + 2;
 
   const bool stalled = stall_test != 0; // test switch: the path of a wait that ran out, with nothing in flight
-  const auto copy_block = [&](int st, int b, int tile) {
-    const uint32_t dst = smem_u32(stages + st * size_t(S::kStageBytes));
-    mbar_expect(full + 8 * st, S::kStageBytes);
-    tma_load_2d(dst, &tm_a, b * kScaleBlock, tile / tiles_n * kTileM, full + 8 * st);
-    tma_load_2d(dst + kTileABytes, &tm_w, b * kScaleBlock, tile % tiles_n * TN, full + 8 * st);
-  };
   // Scales of 16 blocks along k from b on: lane = block and one of four rows
   // (two warps), rows and blocks out of range count nothing.
   const int quarter = (warp - kScaleWarp) * 2 + lane / kScaleChunk, at = lane % kScaleChunk;
@@ -494,17 +486,17 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
     uint64_t sum[S::kCols / 2];
     uint32_t d[2][32];
     bool alive = !stalled;
-    int left = first < tiles ? ((tiles - 1 - first) / stride + 1) * (kb1 - kb0) : 0; // accumulators still to add
-    int acc = 0, chunk = 0; // accumulator in turn, scale buffers taken so far
+    const int sets = (kb1 - kb0 + S::kPair - 1) / S::kPair;                       // of accumulators a tile
+    int left = first < tiles ? ((tiles - 1 - first) / stride + 1) * sets : 0; // still to add
+    int acc = 0, chunk = 0; // set in turn, scale buffers taken so far
     uint32_t parity = 0;    // of the ring's round
-    // The first columns of the accumulator in turn, once it is ready, on their way to registers.
+    // The first columns of the set in turn, once it is ready, on their way to registers.
     const auto begin = [&] {
       alive = wait_warp(ready + 8 * acc, parity, abort_s);
       fence_after();
-      if (alive) tmem_issue32(from + acc * TN, d[0]);
+      if (alive) tmem_issue32(from + acc * (S::kPair * TN), d[0]);
     };
-    constexpr bool kAhead = S::kCols % 64 == 0; // an accumulator ends in d[1]: the next can begin in d[0]
-    if (kAhead && alive && left) begin();
+    if (alive && left) begin();
     for (int tile = first; tile < tiles && alive; tile += stride) {
 #pragma unroll
       for (int j = 0; j < S::kCols / 2; ++j) sum[j] = 0;
@@ -512,25 +504,35 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
         const int buf = chunk % 2;
         alive = wait_warp(sfull + 8 * buf, (chunk / 2) & 1, abort_s);
         const float *sa = scales_a + buf * kScaleChunk * kTileM + row, *sw = scales_w + buf * kScaleChunk * S::kGroups + group;
-        for (int b = min(kScaleChunk, kb1 - c); b > 0 && alive; --b, sa += kTileM, sw += S::kGroups) {
-          const uint64_t scale = pair(__fmul_rn(*sa, *sw));
-          if (!kAhead) begin();
-          if (!alive) break;
+        for (int b = min(kScaleChunk, kb1 - c); b > 0 && alive; b -= S::kPair) {
+          const uint32_t at = from + acc * (S::kPair * TN);
 #pragma unroll
-          for (int j = 0; j < S::kCols; j += 32) {
-            tmem_wait32(d[j / 32 % 2]);
-            if (j + 32 < S::kCols) {
-              tmem_issue32(from + acc * TN + j + 32, d[(j / 32 + 1) % 2]);
-            } else { // all of it is in registers
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(taken + 8 * acc);
-              acc = acc + 1 == S::kAccs ? 0 : acc + 1;
-              parity ^= acc == 0;
-              if (--left && kAhead) begin();
+          for (int u = 0; u < S::kPair; ++u, sa += kTileM, sw += S::kGroups) {
+            if (u >= b) continue;
+            const uint64_t scale = pair(__fmul_rn(*sa, *sw));
+#pragma unroll
+            for (int j = 0; j < S::kCols; j += 32) {
+              const int q = (u * S::kCols + j) / 32 % 2;
+              // Set taken: all of it is in registers; the next begins in d[0], which must be free.
+              const auto next_set = [&] {
+                if (--left) begin();
+              };
+              tmem_wait32(d[q]);
+              const bool last = j + 32 == S::kCols && u + 1 >= min(b, S::kPair);
+              if (!last) {
+                tmem_issue32(at + u * TN + (j + 32 < S::kCols ? j + 32 : TN), d[1 - q]);
+              } else {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(taken + 8 * acc);
+                acc = acc + 1 == S::kAccs ? 0 : acc + 1;
+                parity ^= acc == 0;
+                if (q == 1) next_set();
+              }
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) fma2(sum[(j + i) / 2], d[q][i], d[q][i + 1], scale);
+              if (last && q == 0) next_set();
             }
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) fma2(sum[(j + i) / 2], d[j / 32 % 2][i], d[j / 32 % 2][i + 1], scale);
           }
         }
         __syncwarp();
@@ -562,11 +564,19 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
       bool ok = true;
       int it = 0;
       for (int tile = first; tile < tiles && ok; tile += stride) {
-        for (int b = kb0; b < kb1; ++b, ++it) {
+        for (int b = kb0; b < kb1; b += S::kPair, ++it) {
           const int st = it % S::kStages;
           if (it >= S::kStages) ok = wait_warp(empty + 8 * st, (it / S::kStages - 1) & 1, abort_s);
           if (!ok) break;
-          if (elect()) copy_block(st, b, tile);
+          if (elect()) {
+            const int blocks = min(S::kPair, kb1 - b);
+            mbar_expect(full + 8 * st, blocks * S::kBlockBytes);
+            for (int u = 0; u < blocks; ++u) {
+              const uint32_t dst = smem_u32(stages + st * size_t(S::kStageBytes) + u * S::kBlockBytes);
+              tma_load_2d(dst, &tm_a, (b + u) * kScaleBlock, tile / tiles_n * kTileM, full + 8 * st);
+              tma_load_2d(dst + kTileABytes, &tm_w, (b + u) * kScaleBlock, tile % tiles_n * TN, full + 8 * st);
+            }
+          }
           __syncwarp();
         }
       }
@@ -579,7 +589,7 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
       int it = 0;
       const uint64_t desc_a = sw128_desc(smem_u32(stages)), desc_w = sw128_desc(smem_u32(stages) + kTileABytes);
       for (int tile = first; tile < tiles && ok; tile += stride) {
-        for (int b = kb0; b < kb1; ++b, ++it) {
+        for (int b = kb0; b < kb1; b += S::kPair, ++it) {
           const int st = it % S::kStages, acc = it % S::kAccs;
           ok = wait_warp(full + 8 * st, (it / S::kStages) & 1, abort_s);
           if (ok && it >= S::kAccs) ok = wait_warp(taken + 8 * acc, (it / S::kAccs - 1) & 1, abort_s);
@@ -588,8 +598,14 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
           if (elect()) {
             const uint64_t at = uint64_t(st) * (S::kStageBytes >> 4); // descriptors count 16 bytes
 #pragma unroll
-            for (int j = 0; j < kScaleBlock / 32; ++j)
-              mma_f8<TN>(tmem + acc * TN, desc_a + at + 2 * j, desc_w + at + 2 * j, j > 0);
+            for (int u = 0; u < S::kPair; ++u) {
+              if (b + u >= kb1) continue;
+#pragma unroll
+              for (int j = 0; j < kScaleBlock / 32; ++j) {
+                const uint64_t off = at + u * (S::kBlockBytes >> 4) + 2 * j;
+                mma_f8<TN>(tmem + (acc * S::kPair + u) * TN, desc_a + off, desc_w + off, j > 0);
+              }
+            }
             mma_commit(empty + 8 * st);
             mma_commit(ready + 8 * acc);
           }
@@ -713,16 +729,17 @@ DeviceSetup &setup() {
     configure<128>();
     configure<256>();
     cudaFuncAttributes fa;
-    NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec<1>)); // loads the kernels
-    NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec<2>));
-    NGB_CUDA(cudaFuncGetAttributes(&fa, k_block_vec<4>));
+    for (const void *f : {reinterpret_cast<const void *>(k_block_vec<1, 4, 1>), reinterpret_cast<const void *>(k_block_vec<1, 1, 5>),
+                          reinterpret_cast<const void *>(k_block_vec<2, 4, 1>), reinterpret_cast<const void *>(k_block_vec<4, 2, 1>),
+                          reinterpret_cast<const void *>(k_block_vec<4, 1, 2>)})
+      NGB_CUDA(cudaFuncGetAttributes(&fa, f)); // loads the kernel
     NGB_CUDA(cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device));
     d.clusters[0] = d.sms;
     for (int i = 1; i < 4; ++i) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute attr[1];
-      cluster_config(cfg, attr, 1 << i, 1 << i, TcShape<128>::kThreads, TcShape<128>::kSmem);
-      NGB_CUDA(cudaOccupancyMaxActiveClusters(&d.clusters[i], k_block_tc<128, float>, &cfg));
+      cluster_config(cfg, attr, 1 << i, 1 << i, TcShape<64>::kThreads, TcShape<64>::kSmem);
+      NGB_CUDA(cudaOccupancyMaxActiveClusters(&d.clusters[i], k_block_tc<64, float>, &cfg));
     }
     int *host = nullptr;
     NGB_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&host), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
@@ -746,47 +763,71 @@ int take_stall() {
   return k > 0 ? 1 : 0;
 }
 
-template <int NT> void launch_vec(const BlockMatmulArgs &a, cudaStream_t s) {
+template <int NT, int AHEAD, int CTAS> void launch_vec(const BlockMatmulArgs &a, cudaStream_t s) {
   const int tiles_n = (a.n + 15) / 16;
-  k_block_vec<NT><<<tiles_n * ((a.m + 8 * NT - 1) / (8 * NT)), 32 * kVecWarps, 0, s>>>(a, tiles_n);
+  k_block_vec<NT, AHEAD, CTAS><<<tiles_n * ((a.m + 8 * NT - 1) / (8 * NT)), 32 * kVecWarps, 0, s>>>(a, tiles_n);
 }
 
 template <int TN> void launch_tc(const BlockMatmulArgs &a, int splits, DeviceSetup &d, cudaStream_t s) {
   CUtensorMap tm_a, tm_w;
   if (!make_map(&tm_a, a.a, a.m, a.k, a.lda, kTileM) || !make_map(&tm_w, a.w, a.n, a.k, a.ldw, TN))
     throw std::runtime_error("Cannot describe an 8-bit matrix to the copy engine");
-  const int tiles_n = (a.n + TN - 1) / TN, tiles = tiles_n * ((a.m + kTileM - 1) / kTileM);
+  const long tiles_n = (a.n + TN - 1) / TN, tiles = tiles_n * ((a.m + kTileM - 1) / kTileM);
+  if (tiles > INT_MAX / kMaxSplits) throw std::invalid_argument("Matrix size out of range");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  cluster_config(cfg, attr, splits == 1 ? std::min(tiles, d.sms) : tiles * splits, splits, TcShape<TN>::kThreads,
+  cluster_config(cfg, attr, int(splits == 1 ? std::min(tiles, long(d.sms)) : tiles * splits), splits, TcShape<TN>::kThreads,
                  TcShape<TN>::kSmem);
   cfg.stream = s;
   const auto kernel = a.type == Elem::f32    ? k_block_tc<TN, float>
                       : a.type == Elem::bf16 ? k_block_tc<TN, __nv_bfloat16>
                                              : k_block_tc<TN, __half>;
-  NGB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_w, a, splits, tiles_n, tiles, vector_rows(a), d.err_dev,
+  NGB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_w, a, splits, int(tiles_n), int(tiles), vector_rows(a), d.err_dev,
                               take_stall()));
 }
 
-// Tile width and k split: the shape with the least estimated time.  A CTA's
-// time is its blocks, each bound by the larger of its MMAs and its bytes from
-// L2, plus a start; a split adds its exchange.
+// The launch with the least estimated time, in microseconds.  The estimates
+// are lines fitted to measured times (sizes 1..8192 x 200..8192 x 100..6400,
+// fp32 result, operands from memory); a sample, estimate / measured:
+//   32 x 928 x 768     vec<2> 2.4 / 2.4, tc<32> 5.7 / 5.6    few tiles: latency
+//   256 x 768 x 3200   tc<64>, 4 splits 8.1 / 8.2, tc<32> 9.2 / 9.2
+//   1 x 8192 x 4096    vec<1> one block ahead 10.4 / 10.3, four ahead 13.9
+//   8192 x 8192 x 4096 tc<256> 253 / 255, tc<128> 316 / 320
 struct Plan {
+  int vec; // rows of a a CTA of k_block_vec takes / 8; 0: k_block_tc with the two below
   int tn, splits;
 };
 Plan plan(const BlockMatmulArgs &a, const DeviceSetup &d) {
-  const long kb = (a.k + kScaleBlock - 1) / kScaleBlock, tiles_m = (a.m + kTileM - 1) / kTileM;
-  Plan best{128, 1};
+  const double kb = (a.k + kScaleBlock - 1) / kScaleBlock;
+  Plan best{0, 256, 1};
   double least = 1e30;
-  for (int tn : {32, 64, 128, 256}) {
-    const long tiles = tiles_m * ((a.n + tn - 1) / tn);
-    const double block = std::max(2.0 * tn, (kTileABytes + tn * 128) / 80.0);
+  const auto offer = [&](double t, Plan p) {
+    if (t < least) least = t, best = p;
+  };
+  // k_block_vec: a start, and the rounds of a warp's loads; beyond a CTA an SM
+  // the SM's share of the bytes.
+  const double rounds = std::ceil(kb / kVecWarps);
+  for (int nt : {1, 2, 4}) {
+    const double load = std::ceil(a.n / 16.0) * std::ceil(a.m / (8.0 * nt)) / d.sms;
+    const bool one = load <= 1;
+    if (nt == 1) offer(one ? 1.7 + 0.45 * rounds : 1.5 + 0.8 * rounds * std::max(1.0, 0.8 * load), {1, 0, 0});
+    if (nt == 2) offer(1.7 + 0.67 * rounds * (one ? 1 : 1.6 * load), {2, 0, 0});
+    if (nt == 4) offer(1.85 + 1.08 * rounds * (one ? 1 : 1.3 * load), {4, 0, 0});
+  }
+  // k_block_tc: a start, a tile's blocks, and for each further tile of a CTA
+  // its blocks (their bytes now compete) and its stores.
+  static constexpr struct {
+    int tn;
+    double start, block;
+  } kShapes[] = {{32, 4.6, 0.185}, {64, 5.4, 0.215}, {128, 6.2, 0.25}, {256, 7.7, 0.39}};
+  for (const auto &shape : kShapes) {
+    const double tiles = std::ceil(a.m / double(kTileM)) * std::ceil(a.n / double(shape.tn));
     for (int i = 0; i < 4; ++i) {
       const int splits = 1 << i;
-      if (splits > 1 && (splits > kb || tn > 128 || tiles > d.clusters[i])) continue;
-      const long waves = (tiles + d.clusters[i] - 1) / d.clusters[i];
-      const double t = 2500 + double(waves) * ((kb + splits - 1) / splits * block + 3.0 * tn) + (splits > 1 ? 1500 + 4.0 * tn : 0);
-      if (t < least) least = t, best = {tn, splits};
+      if (splits > 1 && (splits > kb || shape.tn >= 128 || tiles > d.clusters[i])) continue;
+      const double blocks = std::ceil(kb / splits) * shape.block, more = std::ceil(tiles / d.clusters[i]) - 1;
+      offer(shape.start + blocks + more * (1.15 * blocks + 0.5 + 0.012 * shape.tn) + (splits > 1 ? 1.2 : 0),
+            {0, shape.tn, splits});
     }
   }
   return best;
@@ -805,15 +846,17 @@ void check_block_matmul_errors(int device) {
 
 void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s) {
   DeviceSetup &d = setup();
-  // Few rows are bound by the weights' bytes, and by latency.
-  if (a.m <= 16) {
-    if (a.m <= 8)
-      launch_vec<1>(a, s);
+  const Plan p = plan(a, d);
+  if (p.vec) {
+    const bool one = long((a.n + 15) / 16) * ((a.m + 8 * p.vec - 1) / (8 * p.vec)) <= d.sms; // a CTA an SM at most
+    if (p.vec == 1)
+      one ? launch_vec<1, 4, 1>(a, s) : launch_vec<1, 1, 5>(a, s);
+    else if (p.vec == 2)
+      launch_vec<2, 4, 1>(a, s);
     else
-      launch_vec<2>(a, s);
+      one ? launch_vec<4, 2, 1>(a, s) : launch_vec<4, 1, 2>(a, s);
     return;
   }
-  const Plan p = plan(a, d);
   if (p.tn == 32)
     launch_tc<32>(a, p.splits, d, s);
   else if (p.tn == 64)
