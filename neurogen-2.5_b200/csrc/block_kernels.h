@@ -13,6 +13,8 @@ constexpr int kScaleBlock = 128;
 
 // Element types of the operators' 16- and 32-bit arrays (NG_F32, NG_BF16, NG_F16).
 enum class Elem : int { f32 = 0, bf16 = 1, f16 = 2 };
+inline long block_row_bytes(long cols) { return (cols + 15) / 16 * 16; }
+inline long scale_blocks(long n) { return (n + kScaleBlock - 1) / kScaleBlock; }
 inline size_t elem_size(Elem t) { return t == Elem::f32 ? 4 : 2; }
 
 struct QuantArgs {
@@ -26,6 +28,10 @@ struct QuantArgs {
   float *scale;
 };
 void launch_block_quantize(const QuantArgs &a, cudaStream_t s);
+// Loads these kernels and sets up the product on the current device, so that
+// no later launch does (it allocates, and may load code): once per device,
+// outside any stream capture.
+void preload_block_kernels();
 
 // y[m][n] = sum_b a_scale[m][b] w_scale[n / 128][b] sum_{k in block b} a[m][k] w[n][k]
 //           + bias[n] + add_scale * add[m][n]

@@ -835,6 +835,13 @@ Plan plan(const BlockMatmulArgs &a, const DeviceSetup &d) {
 
 } // namespace
 
+void preload_quantize_kernels(); // block_quant.cu
+
+void preload_block_kernels() {
+  setup();
+  preload_quantize_kernels();
+}
+
 void check_block_matmul_errors(int device) {
   if (device < 0 || device >= kMaxDevices) return;
   int *err = g_setup[device].err;

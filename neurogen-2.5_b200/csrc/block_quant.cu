@@ -9,6 +9,7 @@
 // scale, a block with an infinity an infinite scale and NaN in its place, so
 // that every product with it is NaN.
 #include "block_kernels.h"
+#include "common.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -137,7 +138,20 @@ template <class T> void launch_typed(const QuantArgs &a, cudaStream_t s) {
   }
 }
 
+template <class T> void preload_typed() {
+  cudaFuncAttributes fa;
+  for (const void *f : {reinterpret_cast<const void *>(k_quant_rows<T, true>), reinterpret_cast<const void *>(k_quant_rows<T, false>),
+                        reinterpret_cast<const void *>(k_quant_tiles<T, true>), reinterpret_cast<const void *>(k_quant_tiles<T, false>)})
+    NGB_CUDA(cudaFuncGetAttributes(&fa, f));
+}
+
 } // namespace
+
+void preload_quantize_kernels() {
+  preload_typed<float>();
+  preload_typed<__nv_bfloat16>();
+  preload_typed<__half>();
+}
 
 void launch_block_quantize(const QuantArgs &a, cudaStream_t s) {
   if (a.type == Elem::f32)

@@ -159,7 +159,7 @@ void *ng_pool_create(void *engine, int batch) {
     pool->hidden.reset(size_t(batch) * e->config.width * 4);
     pool->act.reset(size_t(batch) * 4);
     pool->parents.reset(size_t(batch) * sizeof(int));
-    pool->sc.ensure(m.dims, batch, m.tc_proj);
+    pool->sc.ensure(m.dims, batch, m.tc_proj, m.fp8_proj);
     NGB_CUDA(cudaStreamCreateWithFlags(&pool->stream, cudaStreamNonBlocking));
     return pool.release();
   });

@@ -58,8 +58,8 @@ float *scratch_address(int device) {
 
 // Offsets (in floats, 256-byte aligned) of one batch-1 step's buffers.
 struct StepLayout {
-  size_t state, token, h, hraw, vin, fb, tr, feat, cnt, logits, hidden, act, total;
-  explicit StepLayout(const LangDims &d) {
+  size_t state, token, h, hraw, vin, fb, tr, feat, cnt, logits, hidden, act, x_q, x_scale, total;
+  StepLayout(const LangDims &d, bool fp8_proj) {
     size_t at = 0;
     auto take = [&](size_t count) {
       const size_t off = at;
@@ -78,6 +78,8 @@ struct StepLayout {
     logits = take(kVocab);
     hidden = take(size_t(d.w));
     act = take(1);
+    x_q = take(fp8_proj ? block_row_bytes(d.kmax()) / 4 : 0); // 8-bit projections only
+    x_scale = take(fp8_proj ? scale_blocks(d.kmax()) : 0);
     total = at;
   }
 };
@@ -101,7 +103,7 @@ extern "C" int ng_step_static(void *p, int token, const float *state, size_t sta
     DeviceModel &m = e.device();
     if (m.device < 0 || m.device >= kMaxDevices) throw std::runtime_error("CUDA device index out of range");
     std::lock_guard<std::mutex> scratch_lock(g_scratch_mutex[m.device]);
-    const StepLayout L(m.dims);
+    const StepLayout L(m.dims, m.fp8_proj);
     if (L.total > kStepScratchFloats)
       throw std::invalid_argument("ng_step_static: this model needs " + std::to_string(L.total) +
                                   " floats of device working memory, more than the fixed " +
@@ -110,6 +112,10 @@ extern "C" int ng_step_static(void *p, int token, const float *state, size_t sta
     float *base = scratch_address(m.device);
     ScratchView v{base + L.h, base + L.hraw, base + L.vin, base + L.fb, base + L.tr, base + L.feat,
                   reinterpret_cast<int *>(base + L.cnt)};
+    if (m.fp8_proj) {
+      v.x_q = reinterpret_cast<uint8_t *>(base + L.x_q);
+      v.x_scale = base + L.x_scale;
+    }
     float *d_state = base + L.state, *d_logits = base + L.logits, *d_hidden = base + L.hidden,
           *d_act = base + L.act;
     int *d_token = reinterpret_cast<int *>(base + L.token);

@@ -80,7 +80,7 @@ LangDims::LangDims(const EngineConfig &cfg, const CorticalColumnV2 &col)
   S = static_cast<long>(R) * RS;
 }
 
-void Scratch::ensure(const LangDims &d, int batch, bool tc_proj) {
+void Scratch::ensure(const LangDims &d, int batch, bool tc_proj, bool fp8_proj) {
   if (batch <= capacity) return;
   const size_t B = batch;
   h.reset(B * d.w * 4);
@@ -99,9 +99,12 @@ void Scratch::ensure(const LangDims &d, int batch, bool tc_proj) {
   h_hi.reset(B * d.w * 4);
   h_lo.reset(B * d.w * 4);
   if (tc_proj) {
-    const size_t kmax = std::max<size_t>(d.w, size_t(d.c) * d.n_out * 2);
-    x_hi.reset(B * kmax * 4);
-    x_lo.reset(B * kmax * 4);
+    x_hi.reset(B * d.kmax() * 4);
+    x_lo.reset(B * d.kmax() * 4);
+  }
+  if (fp8_proj) {
+    x_q.reset(B * block_row_bytes(d.kmax()));
+    x_scale.reset(B * scale_blocks(d.kmax()) * 4);
   }
   capacity = batch;
 }
@@ -177,6 +180,18 @@ DeviceModel::DeviceModel(const EngineConfig &cfg, const CorticalColumnV2 &col, c
     lo_dev = upload(lo);
   };
   tc_proj = projection_tc_enabled();
+  fp8_proj = projection_fp8_enabled();
+  if (fp8_proj) preload_block_kernels();
+  // 8-bit form of a row-major fp32 matrix on the device.
+  auto quantize_weights = [](const DeviceBuffer &w, long M, long K, BlockWeights &to) {
+    to.ld = block_row_bytes(K);
+    to.q.reset(M * to.ld);
+    to.scale.reset(scale_blocks(M) * scale_blocks(K) * 4);
+    launch_block_quantize({w.as<float>(), Elem::f32, nullptr, M, K, K, kScaleBlock, to.q.as<uint8_t>(), to.ld,
+                           to.scale.as<float>()},
+                          nullptr);
+    NGB_CUDA(cudaGetLastError());
+  };
 
   const float *p = data;
   auto take = [&](size_t count) {
@@ -204,15 +219,18 @@ DeviceModel::DeviceModel(const EngineConfig &cfg, const CorticalColumnV2 &col, c
     g.in_wp = upload(to_panels(in_w, c * d.n_in, w));
     g.in_wr = upload(in_w, c * d.n_in * w);
     if (tc_proj) split_upload(in_w, c * d.n_in * w, g.in_hi, g.in_lo);
+    if (fp8_proj) quantize_weights(g.in_wr, c * d.n_in, w, g.in_q);
     g.in_b = upload(take(c * d.n_in), c * d.n_in);
     const float *fb_w = take(c * d.n_fb * w);
     g.fb_wp = upload(to_panels(fb_w, c * d.n_fb, w));
     g.fb_wr = upload(fb_w, c * d.n_fb * w);
     if (tc_proj) split_upload(fb_w, c * d.n_fb * w, g.fb_hi, g.fb_lo);
+    if (fp8_proj) quantize_weights(g.fb_wr, c * d.n_fb, w, g.fb_q);
     const float *out_w = take(w * c * d.n_out * 2);
     g.out_wp = upload(to_panels(out_w, w, c * d.n_out * 2));
     g.out_wr = upload(out_w, w * c * d.n_out * 2);
     if (tc_proj) split_upload(out_w, w * c * d.n_out * 2, g.out_hi, g.out_lo);
+    if (fp8_proj) quantize_weights(g.out_wr, w, c * d.n_out * 2, g.out_q);
     g.out_b = upload(take(w), w);
     g.norm_w = upload(take(w), w);
     g.norm_b = upload(take(w), w);
@@ -226,6 +244,7 @@ DeviceModel::DeviceModel(const EngineConfig &cfg, const CorticalColumnV2 &col, c
   head_wr = upload(head_w, size_t(kVocab) * w);
   split_upload(head_w, size_t(kVocab) * w, head_hi, head_lo);
   head_b = upload(take(kVocab), kVocab);
+  if (fp8_proj) NGB_CUDA(cudaDeviceSynchronize()); // the weights' 8-bit forms, made on the default stream
   NGB_CUDA(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
   NGB_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&readout_err), sizeof(int), cudaHostAllocMapped));
   *readout_err = 0;
@@ -241,6 +260,7 @@ DeviceModel::~DeviceModel() {
 // lost, but the sessions' state does not depend on the readout, so the next
 // step on this engine runs normally.
 void DeviceModel::check_device_errors() const {
+  if (fp8_proj) check_block_matmul_errors(device);
   if (readout_err && *reinterpret_cast<volatile int *>(readout_err)) {
     *reinterpret_cast<volatile int *>(readout_err) = 0;
     throw std::runtime_error("Readout kernel timed out waiting for its tensor-core pipeline");
@@ -264,7 +284,18 @@ void DeviceModel::enqueue_view(int B, const int *d_tokens, const float *d_inputs
   // input split into tf32 hi / lo, then the readout kernel with the
   // projection's weights; the exact sequential kernel otherwise.
   const bool tc_proj_here = tc_proj && B >= 2 && sc.x_hi && sc.x_lo;
-  auto project = [&](const ProjArgs &pa, const DeviceBuffer &w_hi, const DeviceBuffer &w_lo) {
+  // In 8 bits (NEUROGEN_PROJECTION=fp8): the input quantised, then the product
+  // with the weights quantised at load; bias and memory term are its epilogue.
+  if (fp8_proj && !(sc.x_q && sc.x_scale)) throw std::logic_error("8-bit projections need their working memory");
+  auto project = [&](const ProjArgs &pa, const DeviceBuffer &w_hi, const DeviceBuffer &w_lo, const BlockWeights &w_q) {
+    if (fp8_proj) {
+      const long ldq = block_row_bytes(pa.K);
+      launch_block_quantize({pa.x, Elem::f32, pa.xidx, B, pa.K, pa.ldx, 1, sc.x_q, ldq, sc.x_scale}, st);
+      launch_block_matmul({sc.x_q, ldq, sc.x_scale, w_q.q.as<uint8_t>(), w_q.ld, w_q.scale.as<float>(), pa.bias, pa.addv,
+                           pa.ldadd, 0.25f, pa.y, Elem::f32, pa.ldy, B, pa.M, pa.K},
+                          st);
+      return;
+    }
     if (tc_proj_here) {
       launch_tf32_split(pa.x, pa.xidx, pa.ldx, pa.K, B, sc.x_hi, sc.x_lo, st);
       ReadoutArgs a{sc.x_hi, sc.x_lo, pa.K, w_hi.as<float>(), w_lo.as<float>(), pa.bias, pa.y, pa.ldy,
@@ -296,8 +327,9 @@ void DeviceModel::enqueue_view(int B, const int *d_tokens, const float *d_inputs
         fa.K = d.w;
         fa.B = B;
       }
-      if (tc_proj_here) {
-        for (int z = 0; z < fb.count; ++z) project(fb.a[z], regions[r0 + z].fb_hi, regions[r0 + z].fb_lo);
+      if (tc_proj_here || fp8_proj) {
+        for (int z = 0; z < fb.count; ++z)
+          project(fb.a[z], regions[r0 + z].fb_hi, regions[r0 + z].fb_lo, regions[r0 + z].fb_q);
       } else {
         launch_projections(fb, st);
       }
@@ -323,7 +355,7 @@ void DeviceModel::enqueue_view(int B, const int *d_tokens, const float *d_inputs
         ia.M = Min;
         ia.K = d.w;
         ia.B = B;
-        project(ia, g.in_hi, g.in_lo);
+        project(ia, g.in_hi, g.in_lo, g.in_q);
       }
       TickArgs ta{};
       ta.rec = g.rec.as<float>();
@@ -370,7 +402,7 @@ void DeviceModel::enqueue_view(int B, const int *d_tokens, const float *d_inputs
       oa.M = d.w;
       oa.K = Kout;
       oa.B = B;
-      project(oa, g.out_hi, g.out_lo);
+      project(oa, g.out_hi, g.out_lo, g.out_q);
       NormArgs na{};
       na.hraw = sc.hraw;
       na.hraw_ld = d.w;
@@ -494,7 +526,7 @@ void NeuralEngine::step_batch(const int *tokens, int batch, const float *state, 
   DeviceModel &m = *impl_;
   NGB_CUDA(cudaSetDevice(m.device));
   Scratch &sc = m.host_scratch;
-  sc.ensure(m.dims, batch, m.tc_proj);
+  sc.ensure(m.dims, batch, m.tc_proj, m.fp8_proj);
   cudaStream_t st = m.stream;
   NGB_CUDA(cudaMemcpyAsync(sc.tokens.as<int>(), tokens, batch * sizeof(int), cudaMemcpyHostToDevice, st));
   NGB_CUDA(cudaMemcpyAsync(sc.state.as<float>(), state, S * batch * 4, cudaMemcpyHostToDevice, st));
@@ -521,7 +553,7 @@ void NeuralEngine::advance_batch(const float *inputs, int batch, const float *st
   DeviceModel &m = *impl_;
   NGB_CUDA(cudaSetDevice(m.device));
   Scratch &sc = m.host_scratch;
-  sc.ensure(m.dims, batch, m.tc_proj);
+  sc.ensure(m.dims, batch, m.tc_proj, m.fp8_proj);
   cudaStream_t st = m.stream;
   NGB_CUDA(cudaMemcpyAsync(sc.inputs.as<float>(), inputs, size_t(batch) * config.width * 4, cudaMemcpyHostToDevice, st));
   NGB_CUDA(cudaMemcpyAsync(sc.state.as<float>(), state, S * batch * 4, cudaMemcpyHostToDevice, st));

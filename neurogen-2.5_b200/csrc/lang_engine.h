@@ -1,10 +1,12 @@
 // Device-resident language model: dims, weights in HBM, scratch, and the
 // launch sequence of one token / one advance for a batch of sessions.
 #pragma once
+#include "block_kernels.h"
 #include "common.h"
 #include "engine/NeuralEngine.h"
 #include "lang_kernels.h"
 
+#include <algorithm>
 #include <string>
 #include <vector>
 
@@ -17,8 +19,16 @@ struct LangDims {
   int c, w, R, T, idle;
   int n;                 // units per region (c*64)
   int n_in, n_fb, n_out; // 12, 29, 50 per column
+  size_t kmax() const { return std::max<size_t>(w, size_t(c) * n_out * 2); } // longest projection input
   long RS;               // floats per region state block: 5n + w
   long S;                // floats per session state: R * RS
+};
+
+// A weight matrix in 8 bits (block_kernels.h): e4m3 bytes [M][ld], fp32 scales
+// of its 128 x 128 blocks.
+struct BlockWeights {
+  DeviceBuffer q, scale;
+  long ld = 0;
 };
 
 struct RegionWeights {
@@ -29,6 +39,7 @@ struct RegionWeights {
   DeviceBuffer in_wr, fb_wr, out_wr;    // the same three row-major (small-batch kernel)
   // tf32 hi / lo splits of the three row-major matrices (tensor-core projections only)
   DeviceBuffer in_hi, in_lo, fb_hi, fb_lo, out_hi, out_lo;
+  BlockWeights in_q, fb_q, out_q;       // the same three in 8 bits (8-bit projections only)
   DeviceBuffer norm_w, norm_b, decay;   // [w]
 };
 
@@ -40,17 +51,20 @@ struct ScratchView {
   int *cnt;
   float *h_hi = nullptr, *h_lo = nullptr; // tf32 split of h for the tensor-core readout, or null
   float *x_hi = nullptr, *x_lo = nullptr; // [B][max K] tf32 split of a projection's input, or null
+  uint8_t *x_q = nullptr;                 // [B][max K, to 16] 8-bit input of a projection, or null
+  float *x_scale = nullptr;               // [B][ceil(max K / 128)] its scales, or null
 };
 
 // Per-call device workspace for `capacity` sessions.
 struct Scratch {
   int capacity = 0;
-  DeviceBuffer h, hraw, vin, fb, tr, feat, cnt, tokens, inputs, state, logits, hidden, act, h_hi, h_lo, x_hi, x_lo;
-  void ensure(const LangDims &d, int batch, bool tc_proj);
+  DeviceBuffer h, hraw, vin, fb, tr, feat, cnt, tokens, inputs, state, logits, hidden, act, h_hi, h_lo, x_hi, x_lo,
+      x_q, x_scale;
+  void ensure(const LangDims &d, int batch, bool tc_proj, bool fp8_proj);
   ScratchView view() const {
     return {h.as<float>(),   hraw.as<float>(), vin.as<float>(),  fb.as<float>(),  tr.as<float>(),
             feat.as<float>(), cnt.as<int>(),    h_hi.as<float>(), h_lo.as<float>(), x_hi.as<float>(),
-            x_lo.as<float>()};
+            x_lo.as<float>(), x_q.as<uint8_t>(), x_scale.as<float>()};
   }
 };
 
@@ -90,6 +104,9 @@ public:
   // Batched projections on the tensor cores too (NEUROGEN_PROJECTION=tc at
   // model load); the exact sequential projections otherwise.
   bool tc_proj = false;
+  // Every projection in 8 bits (NEUROGEN_PROJECTION=fp8 at model load), at
+  // every batch size; the readout stays as it is.
+  bool fp8_proj = false;
   std::vector<RegionWeights> regions;
   Scratch host_scratch; // used by the host-buffer entry points (under the engine mutex)
   // Error word of the tensor-core readout (pinned, mapped into the device):

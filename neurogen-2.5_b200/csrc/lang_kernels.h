@@ -82,6 +82,9 @@ void launch_tf32_split(const float *x, const int *xidx, long ldx, int K, int B, 
 // True when NEUROGEN_PROJECTION=tc: batched projections (B >= 2) run on the
 // tensor cores as well (split-tf32, not bit-identical to the sequential sum).
 bool projection_tc_enabled();
+// True when NEUROGEN_PROJECTION=fp8: every projection runs on 8-bit operands
+// with block scales (block_matmul.cu).
+bool projection_fp8_enabled();
 void configure_readout_tc();
 const void *readout_tc_kernel();
 // Per-device kernel attributes (dynamic shared memory); call once per device

@@ -272,6 +272,11 @@ bool projection_tc_enabled() {
   return e && std::strcmp(e, "tc") == 0;
 }
 
+bool projection_fp8_enabled() {
+  const char *e = std::getenv("NEUROGEN_PROJECTION");
+  return e && std::strcmp(e, "fp8") == 0;
+}
+
 bool readout_tc_enabled() {
   const char *e = std::getenv("NEUROGEN_READOUT");
   return !(e && std::strcmp(e, "simt") == 0);
