@@ -15,28 +15,27 @@ ELEMENTS = {torch.float32: F32_CODE, torch.bfloat16: 1, torch.float16: 2}
 E4M3 = torch.float8_e4m3fn
 
 
+# The wrappers are on the path of calls that take a few microseconds on the device: each check is one
+# attribute, and results are made by empty_strided, the cheapest of torch's constructors.
+
 def _matrix(x, what):
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError(f'{what} must be a tensor [rows, columns]')
-    if x.device.type != 'cuda':
+    if not x.is_cuda:
         raise ValueError(f'{what} must be on a CUDA device; there is no CPU fallback')
-    if x.shape[1] > 1 and x.stride(1) != 1:
+    shape = x.shape
+    if x.stride(1) != 1 and shape[1] > 1:
         raise ValueError(f'{what} must have adjacent columns')
-    return x.shape
+    return shape
 
 
-def _row_stride(x):
+def _row_stride(x, rows, cols):
     """Elements from a row to the next; a single row has no next."""
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], x.stride(0))
-
-
-def _stride16(x):
-    """Row stride of an 8-bit matrix; a single row takes the next multiple of 16."""
-    return x.stride(0) if x.shape[0] > 1 else -(-x.shape[1] // 16) * 16
+    return x.stride(0) if rows > 1 else cols
 
 
 def _vector(x, shape, dtype, device, what):
-    if (not isinstance(x, torch.Tensor) or x.shape != shape or x.dtype != dtype or x.device != device
+    if (not isinstance(x, torch.Tensor) or x.dtype is not dtype or x.shape != shape or x.device != device
             or not x.is_contiguous()):
         raise ValueError(f'{what} must be contiguous {dtype} {list(shape)} on {device}')
 
@@ -49,17 +48,18 @@ def quantize(x, rows=1):
     rows start on 16-byte boundaries (their row stride is k rounded up to 16).
     """
     m, k = _matrix(x, 'x')
-    if x.dtype not in ELEMENTS:
+    code = ELEMENTS.get(x.dtype)
+    if code is None:
         raise ValueError('x must be float32, bfloat16 or float16')
-    if rows not in (1, BLOCK):
+    if rows != 1 and rows != BLOCK:
         raise ValueError('A scale covers 1 or 128 rows')
     if k < 1:
         raise ValueError('x must have at least one column')
     device = x.device
-    ldq = -(-k // 16) * 16
+    ldq, kb = -(-k // 16) * 16, -(-k // BLOCK)
     q = torch.empty_strided((m, k), (ldq, 1), dtype=E4M3, device=device)
-    scale = torch.empty((-(-m // rows), -(-k // BLOCK)), dtype=torch.float32, device=device)
-    check(library().ng_block_quantize(device.index, x.data_ptr(), ELEMENTS[x.dtype], m, k, _row_stride(x), rows,
+    scale = torch.empty_strided((-(-m // rows), kb), (kb, 1), dtype=torch.float32, device=device)
+    check(library().ng_block_quantize(device.index, x.data_ptr(), code, m, k, _row_stride(x, m, k), rows,
                                       q.data_ptr(), ldq, scale.data_ptr(), stream_of(device)))
     return q, scale
 
@@ -73,31 +73,32 @@ def matmul(a, a_scale, w, w_scale, bias=None, add=None, add_scale=1.0, out_dtype
     """
     m, k = _matrix(a, 'a')
     n, kw = _matrix(w, 'w')
-    if a.dtype != E4M3 or w.dtype != E4M3:
+    if a.dtype is not E4M3 or w.dtype is not E4M3:
         raise ValueError('a and w must be float8_e4m3fn')
     if kw != k:
         raise ValueError(f'a has {k} columns and w {kw}')
     if k < 1 or n < 1:
         raise ValueError('w must not be empty')
-    if out_dtype not in ELEMENTS:
+    code = ELEMENTS.get(out_dtype)
+    if code is None:
         raise ValueError('out_dtype must be float32, bfloat16 or float16')
     device = a.device
     if w.device != device:
         raise ValueError('a and w must be on the same device')
-    kb = -(-k // BLOCK)
+    k16, kb = -(-k // 16) * 16, -(-k // BLOCK)
     _vector(a_scale, (m, kb), torch.float32, device, 'a_scale')
     _vector(w_scale, (-(-n // BLOCK), kb), torch.float32, device, 'w_scale')
     if bias is not None:
         _vector(bias, (n,), torch.float32, device, 'bias')
-    if add is not None and (_matrix(add, 'add') != (m, n) or add.dtype != torch.float32 or add.device != device):
+    if add is not None and (_matrix(add, 'add') != (m, n) or add.dtype is not torch.float32 or add.device != device):
         raise ValueError(f'add must be float32 [{m}, {n}] on {device}')
-    y = torch.empty((m, n), dtype=out_dtype, device=device)
-    check(library().ng_block_matmul(device.index, a.data_ptr(), _stride16(a), a_scale.data_ptr(), w.data_ptr(),
-                                    _stride16(w), w_scale.data_ptr(), m, n, k,
+    y = torch.empty_strided((m, n), (n, 1), dtype=out_dtype, device=device)
+    check(library().ng_block_matmul(device.index, a.data_ptr(), _row_stride(a, m, k16), a_scale.data_ptr(), w.data_ptr(),
+                                    _row_stride(w, n, k16), w_scale.data_ptr(), m, n, k,
                                     None if bias is None else bias.data_ptr(),
                                     None if add is None else add.data_ptr(),
-                                    n if add is None else _row_stride(add), add_scale, y.data_ptr(),
-                                    ELEMENTS[out_dtype], n, stream_of(device)))
+                                    n if add is None else _row_stride(add, m, n), add_scale, y.data_ptr(),
+                                    code, n, stream_of(device)))
     return y
 
 

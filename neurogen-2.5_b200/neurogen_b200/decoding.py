@@ -31,7 +31,8 @@ def beam_select(logits, scores, finished=None, allowed=None, end=None, pad=PAD):
     as finished.  tokens and parents are int32; parents count within the group.
     """
     rows, vocab = _matrix(logits, 'logits')
-    if logits.dtype not in ELEMENTS:
+    code = ELEMENTS.get(logits.dtype)
+    if code is None:
         raise ValueError('logits must be float32, bfloat16 or float16')
     if not isinstance(scores, torch.Tensor) or scores.dim() != 2:
         raise ValueError('scores must be a tensor [groups, beams]')
@@ -56,11 +57,13 @@ def beam_select(logits, scores, finished=None, allowed=None, end=None, pad=PAD):
         raise ValueError('End token outside the vocabulary')
     lib = library()
     need = lib.ng_beam_workspace(groups, beams, vocab)
-    work = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    next_scores = torch.empty(shape, dtype=torch.float32, device=device)
-    tokens, parents = torch.empty((2, groups, beams), dtype=torch.int32, device=device).unbind(0)
-    done = torch.empty(shape, dtype=torch.bool, device=device)
-    check(lib.ng_beam_select(device.index, logits.data_ptr(), ELEMENTS[logits.dtype], _row_stride(logits), groups,
+    work = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device) if need else None
+    stride = (beams, 1)
+    next_scores = torch.empty_strided(shape, stride, dtype=torch.float32, device=device)
+    tokens = torch.empty_strided(shape, stride, dtype=torch.int32, device=device)
+    parents = torch.empty_strided(shape, stride, dtype=torch.int32, device=device)
+    done = torch.empty_strided(shape, stride, dtype=torch.bool, device=device)
+    check(lib.ng_beam_select(device.index, logits.data_ptr(), code, _row_stride(logits, rows, vocab), groups,
                              beams, vocab, scores.data_ptr(), None if finished is None else finished.data_ptr(),
                              None if allowed is None else allowed.data_ptr(), end, pad, next_scores.data_ptr(),
                              tokens.data_ptr(), parents.data_ptr(), done.data_ptr(),
@@ -78,7 +81,7 @@ def reorder(states, parents):
     """
     if not isinstance(states, torch.Tensor) or states.dim() < 1:
         raise ValueError('states must be a tensor [groups * beams, ...]')
-    if states.device.type != 'cuda':
+    if not states.is_cuda:
         raise ValueError('states must be on a CUDA device; there is no CPU fallback')
     if not isinstance(parents, torch.Tensor) or parents.dim() != 2:
         raise ValueError('parents must be a tensor [groups, beams]')
