@@ -22,9 +22,15 @@ template <> __device__ __forceinline__ float to_f32(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
+// fl(amax / 448), at least 2^-126.  The quotient by a constant is one product
+// and its exact remainder's correction (Markstein; equal to the IEEE division
+// for every fp32 amax whose quotient is at least 2^-126).
 __device__ __forceinline__ float block_scale(uint32_t amax_bits) {
-  const float s = __fdiv_rn(__uint_as_float(amax_bits), 448.f);
-  return s < 1.17549435e-38f ? 1.17549435e-38f : s; // a NaN stays
+  constexpr float kInverse = 1.f / 448.f;
+  const float amax = __uint_as_float(amax_bits), q = __fmul_rn(amax, kInverse);
+  const float s = __fmaf_rn(__fmaf_rn(-448.f, q, amax), kInverse, q);
+  if (amax_bits >= 0x7F800000u) return amax; // infinite or NaN
+  return fmaxf(s, 1.17549435e-38f);
 }
 
 // Four values as four e4m3 bytes, round to nearest even.
@@ -35,96 +41,188 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
   return uint32_t(lo) | (uint32_t(hi) << 16);
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-
-// Four consecutive values of a row from column k (values past the row's end
-// are zero).  VEC: the row's start and stride allow one vector load.
-template <class T, bool VEC> __device__ __forceinline__ void load4(const T *row, long k, long cols, float (&v)[4]) {
-  if (VEC && k + 4 <= cols) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 f = *reinterpret_cast<const float4 *>(row + k);
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-    } else {
-      const uint2 u = *reinterpret_cast<const uint2 *>(row + k);
-      const T *e = reinterpret_cast<const T *>(&u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = to_f32<T>(e[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = k + i < cols ? to_f32<T>(row[k + i]) : 0.f;
+// fl(x / scale) for a whole block by one reciprocal and exact remainders
+// (Markstein): with hi + lo = 1 / scale to 2^-47, q = fl(x hi + fl(x lo)) is a
+// neighbour of the quotient, its remainder is exact, and one step from a
+// neighbour by the rounded reciprocal hi gives the correctly rounded quotient.
+// Four operations a value, where the divisions cost more than the block's
+// bytes (a product that divides only near the ties of e4m3 was no faster: bf16
+// ratios are often short, and most warps had one).  The remainders are exact
+// while scale is at least 2^-90 (a quotient below 2^-11, where they might not
+// be, is the byte 0 in any case) and lo is while it is at most 2^90; other
+// blocks divide.  The signs
+// are such that a zero keeps its own.
+struct BlockScale {
+  float scale, hi, lo;
+  bool divide;
+  __device__ __forceinline__ explicit BlockScale(uint32_t amax_bits) {
+    scale = block_scale(amax_bits);
+    hi = __fdiv_rn(1.f, scale);
+    lo = __fmul_rn(__fmaf_rn(-scale, hi, 1.f), hi);
+    divide = !(scale >= 0x1p-90f && scale <= 0x1p90f);
   }
-}
+  __device__ __forceinline__ uint32_t quantize4(const float (&v)[4]) const {
+    float q[4];
+    if (divide) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q[i] = __fdiv_rn(v[i], scale);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        q[i] = __fmaf_rn(v[i], hi, __fmul_rn(v[i], lo));
+        q[i] = __fmaf_rn(-__fmaf_rn(q[i], scale, -v[i]), hi, q[i]);
+      }
+    }
+    return pack_e4m3(q[0], q[1], q[2], q[3]);
+  }
+};
 
-__device__ __forceinline__ void store4(uint8_t *row, long k, long cols, const float (&v)[4], float scale) {
-  const uint32_t u = pack_e4m3(__fdiv_rn(v[0], scale), __fdiv_rn(v[1], scale), __fdiv_rn(v[2], scale),
-                               __fdiv_rn(v[3], scale));
-  if (k + 4 <= cols) {
-    *reinterpret_cast<uint32_t *>(row + k) = u; // the rows start on 16-byte boundaries
-  } else {
+// Sixteen bytes of a row from column k: kN values, zero past the row's end.
+// VEC: the row's start and stride allow one load.  Otherwise four loads of 32
+// bits, or for 16-bit types the one or two aligned 16-byte words that hold
+// them, shifted into place; a word with one byte of the row lies within the
+// row's memory (8000 x 8100 bf16, 128 x 128 blocks: 61 us, with a load a value
+// 86; fp32 74 us with four loads, 112 with shifted words).
+template <class T, bool VEC> struct Chunk {
+  static constexpr int kN = 16 / sizeof(T);
+  union {
+    uint4 words;
+    uint32_t word[4];
+    T raw[kN];
+  };
+  __device__ __forceinline__ Chunk() : words(make_uint4(0, 0, 0, 0)) {}
+  __device__ __forceinline__ void load(const T *row, int k, int cols) {
+    if (k + kN > cols || (!VEC && sizeof(T) == 4)) { // the row's end
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        if (k + i < cols) raw[i] = row[k + i];
+    } else if constexpr (VEC) {
+      words = __ldg(reinterpret_cast<const uint4 *>(row + k));
+    } else {
+      const uintptr_t p = reinterpret_cast<uintptr_t>(row + k);
+      const uint32_t skip = p % 16;
+      const uint4 *from = reinterpret_cast<const uint4 *>(p - skip);
+      const uint4 lo = __ldg(from), hi = __ldg(from + (skip ? 1 : 0));
+      uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      if (skip & 8) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+      }
+      if (skip & 4) {
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) word[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], 8 * (skip & 3));
+    }
+  }
+  // The largest |value|, as bits of its type (their order is the values', a
+  // NaN's above infinity's).  16-bit types: two at a time, one in each half.
+  __device__ __forceinline__ uint32_t amax(uint32_t m) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (k + i < cols) row[k + i] = uint8_t(u >> (8 * i));
+      m = sizeof(T) == 4 ? max(m, word[i] & 0x7FFFFFFFu) : __vmaxu2(m, word[i] & 0x7FFF7FFFu);
+    return m;
+  }
+  __device__ __forceinline__ void store(uint8_t *row, int k, int cols, const BlockScale &s) const {
+    uint32_t u[kN / 4];
+#pragma unroll
+    for (int j = 0; j < kN / 4; ++j) {
+      const float v[4] = {to_f32<T>(raw[4 * j]), to_f32<T>(raw[4 * j + 1]), to_f32<T>(raw[4 * j + 2]), to_f32<T>(raw[4 * j + 3])};
+      u[j] = s.quantize4(v);
+    }
+    if (k + kN <= cols) { // the rows start on 16-byte boundaries
+      if constexpr (kN == 8)
+        *reinterpret_cast<uint2 *>(row + k) = make_uint2(u[0], u[1]);
+      else
+        *reinterpret_cast<uint32_t *>(row + k) = u[0];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kN; ++i)
+        if (k + i < cols) row[k + i] = uint8_t(u[i / 4] >> (8 * (i % 4)));
+    }
+  }
+};
+
+// fp32 bits of an amax over chunks, from the bits of T.
+template <class T> __device__ __forceinline__ uint32_t amax_f32_bits(uint32_t m) {
+  if constexpr (sizeof(T) == 4) {
+    return m;
+  } else {
+    const uint16_t top = uint16_t(max(m & 0xFFFFu, m >> 16));
+    return __float_as_uint(to_f32<T>(*reinterpret_cast<const T *>(&top)));
   }
 }
+template <class T> __device__ __forceinline__ uint32_t amax_join(uint32_t a, uint32_t b) {
+  return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b);
+}
 
-// 1 x 128 blocks: one warp a block, four values a lane.
-template <class T, bool VEC> __global__ void __launch_bounds__(256) k_quant_rows(QuantArgs a, long kb, long blocks) {
-  const int lane = threadIdx.x % 32;
-  const long b = (long(blockIdx.x) * blockDim.x + threadIdx.x) / 32;
+// 1 x 128 blocks: kLanes lanes a block, so that a block's scale and addresses
+// cost a quarter of a warp's instructions (with a warp a block they were most
+// of them: 8192 x 8192 bf16 103 us, 45 now; 2048 x 6400 fp32 17 us, 12.7 now,
+// 5.2 TB/s).
+constexpr int kLanes = 8;
+
+template <class T, bool VEC> __global__ void __launch_bounds__(256) k_quant_rows(QuantArgs a, int kb, int blocks) {
+  using C = Chunk<T, VEC>;
+  constexpr int kChunks = kScaleBlock / (kLanes * C::kN);
+  const long b = (long(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
+  const int lane = threadIdx.x % kLanes, r = b < blocks ? int(b) / kb : 0, c = int(b) - r * kb;
+  const int cols = b < blocks ? int(a.cols) : 0, k = c * kScaleBlock + lane * C::kN; // nothing past the last block
+  const T *row = static_cast<const T *>(a.x) + (a.xidx ? a.xidx[r] : r) * a.ldx;
+  C v[kChunks];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) v[i].load(row, k + i * kLanes * C::kN, cols);
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) m = v[i].amax(m);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o /= 2) m = amax_join<T>(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
   if (b >= blocks) return;
-  const long r = b / kb, c = b % kb, k = c * kScaleBlock + 4 * lane;
-  const T *row = static_cast<const T *>(a.x) + (a.xidx ? long(a.xidx[r]) : r) * a.ldx;
-  float v[4];
-  load4<T, VEC>(row, k, a.cols, v);
-  const uint32_t mine = max(max(abs_bits(v[0]), abs_bits(v[1])), max(abs_bits(v[2]), abs_bits(v[3])));
-  const float scale = block_scale(__reduce_max_sync(0xFFFFFFFFu, mine));
-  if (lane == 0) a.scale[b] = scale;
-  store4(a.q + r * a.ldq, k, a.cols, v, scale);
+  const BlockScale s(amax_f32_bits<T>(m));
+  if (lane == 0) a.scale[b] = s.scale;
+  uint8_t *q = a.q + r * a.ldq;
+#pragma unroll
+  for (int i = 0; i < kChunks; ++i) v[i].store(q, k + i * kLanes * C::kN, cols, s);
 }
 
 // 128 x 128 blocks: one CTA a block, its values in registers between the
-// maximum and the conversion (8 warps x 16 rows, four values a lane and row).
-template <class T, bool VEC> __global__ void __launch_bounds__(256) k_quant_tiles(QuantArgs a, long kb) {
-  constexpr int kWarps = 8, kRows = kScaleBlock / kWarps;
+// maximum and the conversion.
+template <class T, bool VEC> __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 2 : 3) k_quant_tiles(QuantArgs a, int kb) {
+  using C = Chunk<T, VEC>;
+  constexpr int kWarps = 16, kRowLanes = kScaleBlock / C::kN, kRowsAtOnce = 512 / kRowLanes;
+  constexpr int kChunks = kScaleBlock / kRowsAtOnce;
   __shared__ uint32_t part[kWarps];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const long rb = blockIdx.x / kb, c = blockIdx.x % kb, k = c * kScaleBlock + 4 * lane;
-  float v[kRows][4];
-  uint32_t mine = 0;
+  const int rb = blockIdx.x / kb, c = blockIdx.x % kb, k = c * kScaleBlock + threadIdx.x % kRowLanes * C::kN;
+  const long r0 = long(rb) * kScaleBlock + threadIdx.x / kRowLanes;
+  C v[kChunks];
+  uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const long r = rb * kScaleBlock + i * kWarps + warp;
-    if (r < a.rows) {
-      load4<T, VEC>(static_cast<const T *>(a.x) + (a.xidx ? long(a.xidx[r]) : r) * a.ldx, k, a.cols, v[i]);
-    } else {
-      v[i][0] = v[i][1] = v[i][2] = v[i][3] = 0.f;
-    }
+  for (int i = 0; i < kChunks; ++i) {
+    const long r = r0 + i * kRowsAtOnce;
+    if (r < a.rows) v[i].load(static_cast<const T *>(a.x) + (a.xidx ? long(a.xidx[r]) : r) * a.ldx, k, int(a.cols));
   }
 #pragma unroll
-  for (int i = 0; i < kRows; ++i)
-    mine = max(mine, max(max(abs_bits(v[i][0]), abs_bits(v[i][1])), max(abs_bits(v[i][2]), abs_bits(v[i][3]))));
-  mine = __reduce_max_sync(0xFFFFFFFFu, mine);
-  if (lane == 0) part[warp] = mine;
+  for (int i = 0; i < kChunks; ++i) m = v[i].amax(m);
+  m = __reduce_max_sync(0xFFFFFFFFu, amax_f32_bits<T>(m));
+  if (lane == 0) part[warp] = m;
   __syncthreads();
-  mine = part[0];
+  const BlockScale s(__reduce_max_sync(0xFFFFFFFFu, part[lane % kWarps]));
+  if (threadIdx.x == 0) a.scale[long(rb) * kb + c] = s.scale;
 #pragma unroll
-  for (int i = 1; i < kWarps; ++i) mine = max(mine, part[i]);
-  const float scale = block_scale(mine);
-  if (threadIdx.x == 0) a.scale[rb * kb + c] = scale;
-#pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    const long r = rb * kScaleBlock + i * kWarps + warp;
-    if (r < a.rows) store4(a.q + r * a.ldq, k, a.cols, v[i], scale);
+  for (int i = 0; i < kChunks; ++i) {
+    const long r = r0 + i * kRowsAtOnce;
+    if (r < a.rows) v[i].store(a.q + r * a.ldq, k, int(a.cols), s);
   }
 }
 
 template <class T> void launch_typed(const QuantArgs &a, cudaStream_t s) {
-  const long kb = (a.cols + kScaleBlock - 1) / kScaleBlock;
-  const bool vec = reinterpret_cast<uintptr_t>(a.x) % (4 * sizeof(T)) == 0 && a.ldx % 4 == 0;
+  const int kb = int((a.cols + kScaleBlock - 1) / kScaleBlock);
+  const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx * sizeof(T) % 16 == 0;
   if (a.block == 1) {
-    const long blocks = a.rows * kb;
-    const unsigned grid = unsigned((blocks + 7) / 8);
+    const int blocks = int(a.rows * kb); // the callers keep it in 31 bits
+    const unsigned grid = (unsigned(blocks) + 256 / kLanes - 1) / (256 / kLanes);
     if (vec)
       k_quant_rows<T, true><<<grid, 256, 0, s>>>(a, kb, blocks);
     else
@@ -132,9 +230,9 @@ template <class T> void launch_typed(const QuantArgs &a, cudaStream_t s) {
   } else {
     const unsigned grid = unsigned(kb * ((a.rows + kScaleBlock - 1) / kScaleBlock));
     if (vec)
-      k_quant_tiles<T, true><<<grid, 256, 0, s>>>(a, kb);
+      k_quant_tiles<T, true><<<grid, 512, 0, s>>>(a, kb);
     else
-      k_quant_tiles<T, false><<<grid, 256, 0, s>>>(a, kb);
+      k_quant_tiles<T, false><<<grid, 512, 0, s>>>(a, kb);
   }
 }
 
