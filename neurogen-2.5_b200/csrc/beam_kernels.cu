@@ -14,8 +14,13 @@
 // equal totals of two beams to the lower beam.
 //
 // Each row therefore gives a sorted list of its at most `beams` best logits,
-// and a candidate's place among all lists is its place in its own list plus,
-// for every other list, the number of totals before its own (a binary search).
+// and the rows' lists are merged in pairs, one warp a pair.
+//
+// A warp streams over a row, or a part of one.  Its best 32 are kept sorted,
+// one a lane; values above the last that matters gather in shared memory and
+// are sorted and merged in 32 at a time, so that most values cost a comparison.
+// (Taking the best out one by one with warp-wide maxima cost 120 instructions
+// a beam and row: 256 x 8 x 264 12.2 us, @SEL_US@ now.)
 #include "beam_kernels.h"
 
 #include <cuda_bf16.h>
@@ -54,283 +59,342 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// One group's lists: entry p of beam w is (total[w][p], token[w][p]), p < count[w].
-struct Lists {
-  double total[kMaxBeams][kMaxBeams];
-  int token[kMaxBeams][kMaxBeams];
-  int count[kMaxBeams];
-  float score[kMaxBeams];
-  int finished[kMaxBeams];
+// exp of d <= 0 to about 1e-12 of it: 2^n times the Taylor polynomial of
+// degree 10 on |r| <= ln 2 / 2 (its remainder is below 3e-13).  Below -80, and
+// for a NaN, it is 0: against a sum of at least 1 such a term has no bit.  No
+// branches, so that a lane's values overlap.
+__device__ __forceinline__ double exp_below(double x) {
+  const bool counts = x >= -80.0;
+  const double d = counts ? x : 0.0;
+  constexpr double kShift = 6755399441055744.0; // 1.5 * 2^52: the sum's low word is the nearest integer
+  const double t = __fma_rn(d, 1.4426950408889634, kShift);
+  const int n = __double2loint(t);
+  const double r = __fma_rn(-__dsub_rn(t, kShift), 0.6931471805599453, d);
+  double p = 1.0 / 3628800;
+  p = __fma_rn(p, r, 1.0 / 362880);
+  p = __fma_rn(p, r, 1.0 / 40320);
+  p = __fma_rn(p, r, 1.0 / 5040);
+  p = __fma_rn(p, r, 1.0 / 720);
+  p = __fma_rn(p, r, 1.0 / 120);
+  p = __fma_rn(p, r, 1.0 / 24);
+  p = __fma_rn(p, r, 1.0 / 6);
+  p = __fma_rn(p, r, 0.5);
+  p = __fma_rn(p, r, 1.0);
+  p = __fma_rn(p, r, 1.0);
+  return counts ? __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p)) : 0.0;
+}
+
+// Sums of exponentials against the largest logit seen, as its key (0: none).
+struct LogSum {
+  uint32_t top = 0;
+  double sum = 0;
+  __device__ __forceinline__ void raise(uint32_t to) { // to >= top
+    if (to == top) return;
+    if (top) sum = __dmul_rn(sum, exp_below(__dsub_rn(double(logit_of(top)), double(logit_of(to)))));
+    top = to;
+  }
+  __device__ __forceinline__ double term(uint32_t key) const { // key <= top; 0 for no key (it reads as a NaN)
+    return exp_below(__dsub_rn(double(logit_of(key)), double(logit_of(top))));
+  }
+  __device__ __forceinline__ void join_warp() {
+    raise(__reduce_max_sync(kAll, top));
+    sum = warp_sum(sum);
+  }
 };
 
-// Writes the group's results from its lists; all threads of the CTA, after a
-// barrier that makes the lists visible.
-__device__ void place(const BeamArgs &a, int group, const Lists &l) {
-  const int W = a.beams;
-  const long base = long(group) * W;
-  int filled = 0;
-  for (int w = 0; w < W; ++w) filled += l.count[w];
-  for (int i = threadIdx.x; i < W * W; i += blockDim.x) {
-    const int w = i / W, p = i % W;
-    if (p >= l.count[w]) continue;
-    const double mine = l.total[w][p];
-    int rank = p;
-    for (int o = 0; o < W && rank < W; ++o) {
-      if (o == w) continue;
-      // Totals of list o before mine: larger ones, and equal ones of a lower beam.
-      int lo = 0, hi = l.count[o];
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        const double t = l.total[o][mid];
-        if (t > mine || (t == mine && o < w))
-          lo = mid + 1;
-        else
-          hi = mid;
-      }
-      rank += lo;
-    }
-    if (rank >= W) continue;
-    a.next_scores[base + rank] = float(mine);
-    a.tokens[base + rank] = l.token[w][p];
-    a.parents[base + rank] = w;
-    a.next_finished[base + rank] = l.finished[w] || l.token[w][p] == a.end;
-  }
-  for (int j = threadIdx.x; j < W; j += blockDim.x) {
-    if (j < filled) continue; // slots that no candidate fills
-    a.next_scores[base + j] = -INFINITY;
-    a.tokens[base + j] = a.pad;
-    a.parents[base + j] = j;
-    a.next_finished[base + j] = 1;
-  }
+// A value of a row: its key and token, ordered as one number (descending: the
+// larger logit, then the lower token); 0 is none.
+__device__ __forceinline__ uint64_t entry(uint32_t key, uint32_t token) {
+  return key ? (uint64_t(key) << 32) | uint32_t(~token) : 0;
 }
+__device__ __forceinline__ uint32_t entry_key(uint64_t e) { return uint32_t(e >> 32); }
+__device__ __forceinline__ int entry_token(uint64_t e) { return int(~uint32_t(e)); }
 
-// The list of a beam that needs no logits: none, or a finished beam's own.
-// Returns true when the list is done.  One warp.
-__device__ bool settled(const BeamArgs &a, Lists &l, int w, long row) {
+// Of two lanes' entries `apart` apart, the larger to the lower lane or the other way round.
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int apart, bool larger) {
+  const uint64_t o = __shfl_xor_sync(kAll, v, apart);
+  return (v > o) == larger ? v : o;
+}
+// 32 entries, one a lane, in descending order (bitonic sort).
+__device__ __forceinline__ uint64_t sort32(uint64_t v) {
   const int lane = threadIdx.x % 32;
-  const float score = a.scores[row];
-  const int finished = a.finished ? a.finished[row] != 0 : 0;
-  const bool dead = !(fabsf(score) < INFINITY);
-  if (lane == 0) {
-    l.score[w] = score;
-    l.finished[w] = finished;
-    l.count[w] = 0;
-    if (finished && !dead) {
-      l.total[w][0] = double(score);
-      l.token[w][0] = a.pad;
-      l.count[w] = 1;
-    }
-  }
-  return finished || dead;
+#pragma unroll
+  for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+    for (int j = k / 2; j > 0; j /= 2) v = exchange(v, j, ((lane & j) == 0) == ((lane & k) == 0));
+  return v;
+}
+// The best 32 of two sorted lists, sorted.
+__device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b) {
+  const int lane = threadIdx.x % 32;
+  const uint64_t r = __shfl_sync(kAll, b, 31 - lane);
+  a = a > r ? a : r;
+#pragma unroll
+  for (int j = 16; j > 0; j /= 2) a = exchange(a, j, (lane & j) == 0);
+  return a;
 }
 
-// Small vocabularies: one CTA a group, one warp a beam, the row in registers
-// (N values a lane; value i of a lane is token 32 i + lane).
-constexpr int kSmallVocab = 1024;
+// A warp's best entries of what it has seen.
+struct Best {
+  uint64_t mine = 0; // the lane-th best
+  uint64_t bar = 0;  // only entries above it can still matter
+  int held = 0;      // entries waiting in the warp's kWaiting places
+  __device__ __forceinline__ void flush(uint64_t *wait, int beams) {
+    const int lane = threadIdx.x % 32;
+    __syncwarp();
+    const uint64_t v = lane < held ? wait[lane] : 0, later = 32 + lane < held ? wait[32 + lane] : 0;
+    __syncwarp();
+    wait[lane] = later;
+    __syncwarp();
+    held = max(held - 32, 0);
+    mine = merge32(mine, sort32(v));
+    const uint64_t last = __shfl_sync(kAll, mine, beams - 1);
+    bar = bar > last ? bar : last;
+  }
+  __device__ __forceinline__ void push(uint64_t e, uint64_t *wait, int beams) {
+    const unsigned who = __ballot_sync(kAll, e > bar);
+    if (!who) return;
+    if (e > bar) wait[held + __popc(who & ((1u << (threadIdx.x % 32)) - 1u))] = e;
+    held += __popc(who);
+    if (held >= 32) flush(wait, beams);
+  }
+};
 
-template <class T, int N> __global__ void __launch_bounds__(1024) k_beam_small(BeamArgs a) {
-  __shared__ Lists l;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+// Streams over tokens [v0, v1) of a row.  kStep values a lane are in flight;
+// nine cover the byte vocabulary (264) in one step.
+constexpr int kStep = 9;
+template <class T>
+__device__ __forceinline__ void stream_row(const BeamArgs &a, const T *x, int v0, int v1, LogSum &ls, Best &best,
+                                           uint64_t *wait) {
+  const int lane = threadIdx.x % 32;
+  T next[kStep];
+  const auto load = [&](int v) { // past the end: the last value, which is not used
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) next[i] = x[min(v + 32 * i + lane, v1 - 1)];
+  };
+  if (v0 < v1) load(v0);
+  for (int v = v0; v < v1; v += 32 * kStep) {
+    uint32_t key[kStep], top = 0;
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) key[i] = v + 32 * i + lane < v1 ? key_of(to_f32<T>(next[i])) : 0u;
+    if (a.allowed) {
+      uint8_t ok[kStep];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) ok[i] = a.allowed[min(v + 32 * i + lane, v1 - 1)];
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) key[i] = ok[i] ? key[i] : 0u;
+    }
+    if (v + 32 * kStep < v1) load(v + 32 * kStep);
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) top = max(top, key[i]);
+    if (top > ls.top) ls.raise(top);
+    double term[kStep];
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) term[i] = ls.term(key[i]);
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) ls.sum = __dadd_rn(ls.sum, term[i]);
+    if (v == v0) // of the lanes' largest, the beams-th: at least `beams` values reach it
+      best.bar = uint64_t(entry_key(__shfl_sync(kAll, sort32(uint64_t(top) << 32), a.beams - 1))) << 32;
+    if (!__any_sync(kAll, top >= entry_key(best.bar) && top)) continue;
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) best.push(entry(key[i], v + 32 * i + lane), wait, a.beams);
+  }
+  while (best.held) best.flush(wait, a.beams);
+}
+
+// A candidate among all of a group's: its total as a number in the same order
+// (0: none), and where it stands, beam * 32 + place in the beam's list.
+struct Cand {
+  uint64_t key = 0;
+  uint32_t id = kAll;
+};
+__device__ __forceinline__ uint64_t key_of_total(double t) {
+  const uint64_t u = uint64_t(__double_as_longlong(__dadd_rn(t, 0.0))); // -0 is +0
+  return (u >> 63) ? ~u : u | (uint64_t(1) << 63);
+}
+__device__ __forceinline__ double total_of(uint64_t key) {
+  return __longlong_as_double((key >> 63) ? key & ~(uint64_t(1) << 63) : ~key);
+}
+__device__ __forceinline__ bool before(const Cand &a, const Cand &b) {
+  return a.key > b.key || (a.key == b.key && a.id < b.id);
+}
+// The best 32 of two sorted lists, one entry a lane, sorted.
+__device__ __forceinline__ Cand merge_cands(Cand a, const Cand &b) {
+  const int lane = threadIdx.x % 32;
+  Cand o{__shfl_sync(kAll, b.key, 31 - lane), __shfl_sync(kAll, b.id, 31 - lane)};
+  if (before(o, a)) a = o;
+#pragma unroll
+  for (int j = 16; j > 0; j /= 2) {
+    o = {__shfl_xor_sync(kAll, a.key, j), __shfl_xor_sync(kAll, a.id, j)};
+    if (before(o, a) == ((lane & j) == 0)) a = o;
+  }
+  return a;
+}
+
+// A warp's part of shared memory: first the entries it holds back (Best), then
+// its beam's list.
+constexpr int kWaiting = 64;
+union WarpShare {
+  uint64_t wait[kWaiting];
+  struct {
+    uint64_t key[32];
+    uint32_t id[32];
+    int token[32];
+  } list;
+};
+
+// A beam and what becomes of it: alive (its row counts), finished (one
+// candidate of its own) or neither.
+struct Beam {
+  float score;
+  bool finished, exists;
+  __device__ __forceinline__ Beam(const BeamArgs &a, long row)
+      : score(a.scores[row]), finished(a.finished && a.finished[row]), exists(fabsf(score) < INFINITY) {}
+};
+
+// A group's results from its beams' best logits; warp w is beam w, lane its
+// place in the list.  Every warp's entries leave its share of shared memory,
+// whose lists are then merged in pairs; the first warp's is the answer.
+__device__ __forceinline__ void finish_group(const BeamArgs &a, int group, const Beam &beam, const LogSum &ls,
+                                             uint64_t mine, WarpShare *shares) {
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32, W = a.beams;
+  Cand c;
+  int token = a.pad;
+  if (beam.exists && beam.finished) {
+    if (lane == 0) c.key = key_of_total(double(beam.score));
+  } else if (beam.exists && ls.top != 0 && ls.top != kBadKey) {
+    const double lse = __dadd_rn(double(logit_of(ls.top)), log(ls.sum));
+    token = entry_token(mine);
+    if (lane < W && mine) c.key = key_of_total(__dadd_rn(double(beam.score), __dsub_rn(double(logit_of(entry_key(mine))), lse)));
+  }
+  if (c.key) c.id = w * 32 + lane;
+  auto &list = shares[w].list;
+  __syncwarp(); // the share's other use is over
+  list.token[lane] = token;
+  int *done = reinterpret_cast<int *>(shares + W); // of each beam
+  if (lane == 0) done[w] = beam.finished;
+  for (int step = 1; step < W; step *= 2) {
+    if (w % (2 * step) == step) list.key[lane] = c.key, list.id[lane] = c.id;
+    __syncthreads();
+    if (w % (2 * step) == 0 && w + step < W) {
+      const auto &other = shares[w + step].list;
+      c = merge_cands(c, {other.key[lane], other.id[lane]});
+    }
+  }
+  if (w || lane >= W) return;
+  const long at = long(group) * W + lane;
+  if (c.key) {
+    const int parent = c.id / 32, chosen = shares[parent].list.token[c.id % 32];
+    a.next_scores[at] = float(total_of(c.key));
+    a.tokens[at] = chosen;
+    a.parents[at] = parent;
+    a.next_finished[at] = done[parent] || chosen == a.end;
+  } else { // no candidate fills this slot
+    a.next_scores[at] = -INFINITY;
+    a.tokens[at] = a.pad;
+    a.parents[at] = lane;
+    a.next_finished[at] = 1;
+  }
+}
+size_t share_bytes(int beams) { return beams * (sizeof(WarpShare) + sizeof(int)); }
+
+// One launch: one CTA a group, one warp a beam.
+template <class T> __global__ void __launch_bounds__(1024) k_beam_rows(BeamArgs a) {
+  extern __shared__ uint64_t shared[];
+  WarpShare *shares = reinterpret_cast<WarpShare *>(shared);
+  const int w = threadIdx.x / 32;
   const long row = long(blockIdx.x) * a.beams + w;
-  if (!settled(a, l, w, row)) {
-    const T *x = static_cast<const T *>(a.logits) + row * a.ld;
-    uint32_t key[N], best = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int v = 32 * i + lane;
-      key[i] = v < a.vocab && (!a.allowed || a.allowed[v]) ? key_of(to_f32<T>(x[v])) : 0u;
-      best = max(best, key[i]);
-    }
-    uint32_t top = __reduce_max_sync(kAll, best);
-    if (top != 0 && top != kBadKey) {
-      const double m = logit_of(top);
-      double sum = 0;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (key[i]) sum = __dadd_rn(sum, exp(__dsub_rn(double(logit_of(key[i])), m)));
-      const double lse = __dadd_rn(m, log(warp_sum(sum)));
-      const double score = l.score[w];
-      int p = 0;
-      for (; p < a.beams && top != 0; ++p) {
-        // The first token that holds the largest key, then the lane's next best.
-        unsigned token = kAll;
-#pragma unroll
-        for (int i = N - 1; i >= 0; --i)
-          if (key[i] == top) token = 32 * i + lane;
-        const unsigned first = __reduce_min_sync(kAll, token);
-        if (first == token) {
-          best = 0;
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            if (32 * i + lane == int(first)) key[i] = 0;
-            best = max(best, key[i]);
-          }
-        }
-        if (lane == 0) {
-          l.total[w][p] = __dadd_rn(score, __dsub_rn(double(logit_of(top)), lse));
-          l.token[w][p] = int(first);
-        }
-        top = __reduce_max_sync(kAll, best);
-      }
-      if (lane == 0) l.count[w] = p;
-    }
+  const Beam beam(a, row);
+  LogSum ls;
+  Best best;
+  if (beam.exists && !beam.finished) {
+    stream_row<T>(a, static_cast<const T *>(a.logits) + row * a.ld, 0, a.vocab, ls, best, shares[w].wait);
+    ls.join_warp();
   }
-  __syncthreads();
-  place(a, blockIdx.x, l);
+  finish_group(a, blockIdx.x, beam, ls, best.mine, shares);
 }
 
-// Larger vocabularies: each row in up to kSlices slices, one CTA a slice; a
-// slice leaves its largest logit, sum of exponentials and sorted best logits
-// in the workspace, and one CTA a group joins them.
-constexpr int kSliceThreads = 256, kPerThread = 16, kChunk = kSliceThreads * kPerThread;
-constexpr int kSlices = 32;
+// Two launches, where there are too few rows for their length: each row in up
+// to kSlices slices, one CTA a slice; a slice leaves its sum and its sorted
+// best entries in the workspace, and one CTA a group joins them.
+constexpr int kSliceWarps = 8, kSlices = 32;
+constexpr int kRowsVocab = 2048, kManyRows = 1184; // see in_slices
 
 struct Slice {
-  double sum; // of exp(x - largest logit of the slice)
+  double sum;
   uint32_t top;
-  int count;
-  uint64_t best[kMaxBeams]; // key << 32 | ~token: descending, equal keys by token
+  uint64_t best[kMaxBeams];
 };
 
-__host__ __device__ inline int slice_count(int vocab) {
-  const int chunks = (vocab + kChunk - 1) / kChunk;
-  return chunks < kSlices ? chunks : kSlices;
+// One launch serves short rows, and rows enough to give every SM eight warps.
+__host__ __device__ inline bool in_slices(long rows, int vocab) { return vocab > kRowsVocab && rows < kManyRows; }
+// Slices of a row: about four CTAs an SM, none shorter than a warp's step of values for every warp.
+__host__ __device__ inline int slice_count(long rows, int vocab) {
+  const int want = int((4 * 148 + rows - 1) / rows), most = (vocab + 32 * kStep * kSliceWarps - 1) / (32 * kStep * kSliceWarps);
+  const int n = want < most ? want : most;
+  return n < kSlices ? n : kSlices;
 }
 
-template <class T> __global__ void __launch_bounds__(kSliceThreads) k_beam_slice(BeamArgs a) {
-  __shared__ uint64_t lead[kSliceThreads];
-  __shared__ uint64_t kept[kMaxBeams], pool[kMaxBeams * (kPerThread + 1)];
-  __shared__ int pooled;
-  __shared__ double sums[kSliceThreads / 32];
-  const int slices = slice_count(a.vocab), W = a.beams, tid = threadIdx.x;
+template <class T> __global__ void __launch_bounds__(32 * kSliceWarps) k_beam_slice(BeamArgs a, int slices) {
+  __shared__ uint64_t wait[kSliceWarps][kWaiting];
+  __shared__ double sums[kSliceWarps];
+  __shared__ uint32_t tops[kSliceWarps];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const long row = blockIdx.x / slices;
   const int slice = blockIdx.x % slices;
-  Slice *out = static_cast<Slice *>(a.work) + blockIdx.x;
-  const float score = a.scores[row];
-  if (!(fabsf(score) < INFINITY) || (a.finished && a.finished[row])) return; // the row's logits do not count
-  const T *x = static_cast<const T *>(a.logits) + row * a.ld;
-  // Whole chunks to every slice, so that slices differ by one chunk at most.
-  const long chunks = (long(a.vocab) + kChunk - 1) / kChunk;
-  const int c0 = int(slice * chunks / slices), c1 = int((slice + 1) * chunks / slices);
-  uint32_t top = 0; // largest key so far, and the sum of exponentials against it
-  double sum = 0;
-  int held = 0; // entries of kept
-  for (int c = c0; c < c1; ++c) {
-    uint32_t key[kPerThread];
-    uint64_t best = 0;
-    const long v0 = long(c) * kChunk + tid;
-#pragma unroll
-    for (int i = 0; i < kPerThread; ++i) {
-      const long v = v0 + long(i) * kSliceThreads;
-      key[i] = v < a.vocab && (!a.allowed || a.allowed[v]) ? key_of(to_f32<T>(x[v])) : 0u;
-      const uint64_t k = key[i] ? (uint64_t(key[i]) << 32) | uint32_t(~uint32_t(v)) : 0;
-      best = best > k ? best : k;
-    }
-    __syncthreads(); // the previous chunk's pool has been read
-    lead[tid] = best;
-    if (tid == 0) pooled = held;
-    if (tid < held) pool[tid] = kept[tid];
-    __syncthreads();
-    // The threshold: the W-th largest of the threads' leaders (distinct, but
-    // for 0).  At least W values reach it, and only W threads hold such values.
-    int before = 0;
-    for (int i = 0; i < kSliceThreads; ++i) before += lead[i] > best;
-    if (best != 0 && before < W) {
-      // This thread's leader is among the first W: the W-th largest bounds its values.
-      // Every value of the thread may be among the best.
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i) {
-        const long v = v0 + long(i) * kSliceThreads;
-        if (key[i]) pool[atomicAdd(&pooled, 1)] = (uint64_t(key[i]) << 32) | uint32_t(~uint32_t(v));
-      }
-    }
-    uint32_t chunk_top = uint32_t(best >> 32);
-    chunk_top = __reduce_max_sync(kAll, chunk_top);
-    __syncthreads();
-    if (tid % 32 == 0) lead[tid / 32] = chunk_top; // every leader has been compared
-    // The best W of the pool, sorted: each entry's place is the number before it.
-    const int n = pooled;
-    for (int i = tid; i < n; i += kSliceThreads) {
-      const uint64_t k = pool[i];
-      int at = 0;
-      for (int j = 0; j < n; ++j) at += pool[j] > k;
-      if (at < W) kept[at] = k;
-    }
-    __syncthreads();
-    held = min(n, W);
-    uint32_t next = top;
-#pragma unroll
-    for (int i = 0; i < kSliceThreads / 32; ++i) next = max(next, uint32_t(lead[i]));
-    if (next != 0 && next != kBadKey) {
-      const double m = logit_of(next);
-      if (top != 0 && top != next) sum = __dmul_rn(sum, exp(__dsub_rn(double(logit_of(top)), m)));
-#pragma unroll
-      for (int i = 0; i < kPerThread; ++i)
-        if (key[i]) sum = __dadd_rn(sum, exp(__dsub_rn(double(logit_of(key[i])), m)));
-    }
-    top = next;
-  }
-  sum = warp_sum(sum);
-  if (tid % 32 == 0) sums[tid / 32] = sum;
+  const Beam beam(a, row);
+  if (!beam.exists || beam.finished) return; // the row's logits do not count
+  const int part = slice * kSliceWarps + warp, parts = slices * kSliceWarps;
+  LogSum ls;
+  Best best;
+  stream_row<T>(a, static_cast<const T *>(a.logits) + row * a.ld, int(long(part) * a.vocab / parts),
+                int(long(part + 1) * a.vocab / parts), ls, best, wait[warp]);
+  ls.join_warp();
+  __syncwarp();
+  wait[warp][lane] = best.mine;
+  if (lane == 0) sums[warp] = ls.sum, tops[warp] = ls.top;
   __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < kSliceThreads / 32; ++i) sum = __dadd_rn(sum, sums[i]);
-    out->sum = sum;
-    out->top = top;
-    out->count = held;
-  }
-  if (tid < held) out->best[tid] = kept[tid];
+  if (warp) return;
+  for (int i = 1; i < kSliceWarps; ++i) best.mine = merge32(best.mine, wait[i][lane]);
+  LogSum all;
+  if (lane < kSliceWarps) all.sum = sums[lane], all.top = tops[lane];
+  all.join_warp();
+  Slice *out = static_cast<Slice *>(a.work) + blockIdx.x;
+  if (lane < a.beams) out->best[lane] = best.mine;
+  if (lane == 0) out->sum = all.sum, out->top = all.top;
 }
 
-__global__ void __launch_bounds__(1024) k_beam_join(BeamArgs a) {
-  __shared__ Lists l;
-  const int lane = threadIdx.x % 32, w = threadIdx.x / 32, slices = slice_count(a.vocab);
+__global__ void __launch_bounds__(1024) k_beam_join(BeamArgs a, int slices) {
+  extern __shared__ uint64_t shared[];
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
   const long row = long(blockIdx.x) * a.beams + w;
-  if (!settled(a, l, w, row)) {
-    // Lane = slice.
-    const Slice *s = static_cast<const Slice *>(a.work) + row * slices + lane;
-    const uint32_t mine = lane < slices ? s->top : 0u;
-    const uint32_t top = __reduce_max_sync(kAll, mine);
-    if (top != 0 && top != kBadKey) {
-      const double m = logit_of(top);
-      const double part = mine ? __dmul_rn(s->sum, exp(__dsub_rn(double(logit_of(mine)), m))) : 0.0;
-      const double lse = __dadd_rn(m, log(warp_sum(part)));
-      const double score = l.score[w];
-      const int count = lane < slices ? s->count : 0;
-      int used = 0, p = 0;
-      for (; p < a.beams; ++p) {
-        const uint64_t head = used < count ? s->best[used] : 0;
-        const uint32_t key = __reduce_max_sync(kAll, uint32_t(head >> 32));
-        if (key == 0) break;
-        const unsigned token = uint32_t(head >> 32) == key ? ~uint32_t(head) : kAll;
-        const unsigned first = __reduce_min_sync(kAll, token);
-        used += token == first;
-        if (lane == 0) {
-          l.total[w][p] = __dadd_rn(score, __dsub_rn(double(logit_of(key)), lse));
-          l.token[w][p] = int(first);
-        }
-      }
-      if (lane == 0) l.count[w] = p;
+  const Beam beam(a, row);
+  LogSum ls;
+  uint64_t mine = 0;
+  if (beam.exists && !beam.finished) {
+    const Slice *s = static_cast<const Slice *>(a.work) + row * slices;
+    if (lane < slices) ls.top = s[lane].top, ls.sum = s[lane].sum;
+    ls.join_warp();
+    for (int i = 0; i < slices; i += 4) { // four lists' loads in flight together
+      uint64_t e[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) e[j] = i + j < slices && lane < a.beams ? s[i + j].best[lane] : 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (i + j < slices) mine = merge32(mine, e[j]);
     }
   }
-  __syncthreads();
-  place(a, blockIdx.x, l);
+  finish_group(a, blockIdx.x, beam, ls, mine, reinterpret_cast<WarpShare *>(shared));
 }
 
 template <class T> void select_typed(const BeamArgs &a, cudaStream_t s) {
-  if (a.vocab <= kSmallVocab) {
-    const dim3 grid(a.groups), block(32 * a.beams);
-    if (a.vocab <= 128)
-      k_beam_small<T, 4><<<grid, block, 0, s>>>(a);
-    else if (a.vocab <= 288)
-      k_beam_small<T, 9><<<grid, block, 0, s>>>(a);
-    else if (a.vocab <= 512)
-      k_beam_small<T, 16><<<grid, block, 0, s>>>(a);
-    else
-      k_beam_small<T, 32><<<grid, block, 0, s>>>(a);
+  const long rows = long(a.groups) * a.beams;
+  if (in_slices(rows, a.vocab)) {
+    const int slices = slice_count(rows, a.vocab);
+    k_beam_slice<T><<<unsigned(rows * slices), 32 * kSliceWarps, 0, s>>>(a, slices);
+    k_beam_join<<<a.groups, 32 * a.beams, share_bytes(a.beams), s>>>(a, slices);
   } else {
-    k_beam_slice<T><<<unsigned(a.groups) * a.beams * slice_count(a.vocab), kSliceThreads, 0, s>>>(a);
-    k_beam_join<<<a.groups, 32 * a.beams, 0, s>>>(a);
+    k_beam_rows<T><<<a.groups, 32 * a.beams, share_bytes(a.beams), s>>>(a);
   }
 }
 
@@ -376,7 +440,8 @@ template <class U> void reorder_unit(const ReorderArgs &a, cudaStream_t s) {
 } // namespace
 
 size_t beam_workspace(int groups, int beams, int vocab) {
-  return vocab <= kSmallVocab ? 0 : size_t(groups) * beams * slice_count(vocab) * sizeof(Slice);
+  const long rows = long(groups) * beams;
+  return in_slices(rows, vocab) ? size_t(rows) * slice_count(rows, vocab) * sizeof(Slice) : 0;
 }
 
 void launch_beam_select(const BeamArgs &a, cudaStream_t s) {

@@ -153,6 +153,7 @@ int ng_beam_select(int device, const void *logits, int dtype, int64_t ld, int gr
     a.type = elem(dtype);
     require(beams >= 1 && beams <= kMaxBeams, "Beams must be 1..32");
     require(vocab >= 1, "Vocabulary must not be empty");
+    require(vocab <= 1 << 30, "Vocabulary too large");
     require(groups >= 0 && int64_t(groups) * beams <= INT_MAX / 32, "Too many beams in one call");
     require(ld >= vocab, "Row stride smaller than the row");
     require(pad >= 0 && pad < vocab, "Padding token outside the vocabulary");
