@@ -14,7 +14,7 @@
 // equal totals of two beams to the lower beam.
 //
 // Each row therefore gives a sorted list of its at most `beams` best logits,
-// and the rows' lists are merged in pairs, one warp a pair.
+// and the rows' lists are joined (finish_group).
 //
 // A warp streams over a row, or a part of one.  Its best 32 are kept sorted,
 // one a lane; values above the last that matters gather in shared memory and
@@ -39,18 +39,18 @@ template <> __device__ __forceinline__ float to_f32(float v) { return v; }
 template <> __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
 template <> __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
 
-// Logits as unsigned keys in their order; 0 is no candidate (a masked token or
-// -inf), kBadKey a value that leaves the row's distribution undefined.
-constexpr uint32_t kBadKey = 0xFFFFFFFFu;
+// Logits as unsigned keys in their order: the bits, negative ones inverted,
+// from -inf = 0 up.  0 is also a masked token: no candidate.  +inf and NaN (of
+// either sign: the addition, which makes -0 +0, also makes every NaN the same
+// positive one) leave the row's distribution undefined: kBadKey and above.
+constexpr uint32_t kLowest = 0x007FFFFFu, kBadKey = 0xFF800000u - kLowest;
 __device__ __forceinline__ uint32_t key_of(float x) {
-  x = __fadd_rn(x, 0.f); // -0 and +0 are equal logits
-  const uint32_t u = __float_as_uint(x);
-  if (x == -INFINITY) return 0u;
-  if (!(x < INFINITY)) return kBadKey; // +inf or NaN
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  const uint32_t u = __float_as_uint(__fadd_rn(x, 0.f));
+  return (u ^ (uint32_t(int(u) >> 31) | 0x80000000u)) - kLowest;
 }
 __device__ __forceinline__ float logit_of(uint32_t key) {
-  return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+  const uint32_t k = key + kLowest;
+  return __uint_as_float(k ^ (~uint32_t(int(k) >> 31) | 0x80000000u));
 }
 
 __device__ __forceinline__ double warp_sum(double v) {
@@ -59,29 +59,31 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// exp of d <= 0 to about 1e-12 of it: 2^n times the Taylor polynomial of
-// degree 10 on |r| <= ln 2 / 2 (its remainder is below 3e-13).  Below -80, and
-// for a NaN, it is 0: against a sum of at least 1 such a term has no bit.  No
-// branches, so that a lane's values overlap.
-__device__ __forceinline__ double exp_below(double x) {
-  const bool counts = x >= -80.0;
-  const double d = counts ? x : 0.0;
+// exp of N values <= 0, each to about 1e-12 of it: 2^n times the Taylor
+// polynomial of degree 10 on |r| <= ln 2 / 2 (its remainder is below 3e-13).
+// Below -80, and for a NaN, it is 0: against a sum of at least 1 such a term
+// has no bit.  The values go through each step together: a 64-bit operation
+// takes 8 clocks and another can start every second.
+template <int N> __device__ __forceinline__ void exp_below(double (&v)[N]) {
   constexpr double kShift = 6755399441055744.0; // 1.5 * 2^52: the sum's low word is the nearest integer
-  const double t = __fma_rn(d, 1.4426950408889634, kShift);
-  const int n = __double2loint(t);
-  const double r = __fma_rn(-__dsub_rn(t, kShift), 0.6931471805599453, d);
-  double p = 1.0 / 3628800;
-  p = __fma_rn(p, r, 1.0 / 362880);
-  p = __fma_rn(p, r, 1.0 / 40320);
-  p = __fma_rn(p, r, 1.0 / 5040);
-  p = __fma_rn(p, r, 1.0 / 720);
-  p = __fma_rn(p, r, 1.0 / 120);
-  p = __fma_rn(p, r, 1.0 / 24);
-  p = __fma_rn(p, r, 1.0 / 6);
-  p = __fma_rn(p, r, 0.5);
-  p = __fma_rn(p, r, 1.0);
-  p = __fma_rn(p, r, 1.0);
-  return counts ? __hiloint2double(__double2hiint(p) + (n << 20), __double2loint(p)) : 0.0;
+  constexpr double kTaylor[10] = {1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120,
+                                  1.0 / 24,     1.0 / 6,     0.5,        1.0,       1.0};
+  double t[N], p[N];
+  bool counts[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    counts[i] = v[i] >= -80.0;
+    t[i] = __fma_rn(v[i], 1.4426950408889634, kShift);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = __fma_rn(-__dsub_rn(t[i], kShift), 0.6931471805599453, v[i]), p[i] = 1.0 / 3628800;
+#pragma unroll
+  for (int k = 0; k < 10; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = __fma_rn(p[i], v[i], kTaylor[k]);
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    v[i] = counts[i] ? __hiloint2double(__double2hiint(p[i]) + (__double2loint(t[i]) << 20), __double2loint(p[i])) : 0.0;
 }
 
 // Sums of exponentials against the largest logit seen, as its key (0: none).
@@ -90,11 +92,24 @@ struct LogSum {
   double sum = 0;
   __device__ __forceinline__ void raise(uint32_t to) { // to >= top
     if (to == top) return;
-    if (top) sum = __dmul_rn(sum, exp_below(__dsub_rn(double(logit_of(top)), double(logit_of(to)))));
+    double d[1] = {__dsub_rn(double(logit_of(top)), double(logit_of(to)))};
+    exp_below(d);
+    sum = top ? __dmul_rn(sum, d[0]) : 0.0;
     top = to;
   }
-  __device__ __forceinline__ double term(uint32_t key) const { // key <= top; 0 for no key (it reads as a NaN)
-    return exp_below(__dsub_rn(double(logit_of(key)), double(logit_of(top))));
+  // Adds N logits' terms; none above top, -inf for none.  TOGETHER at a time.
+  template <int TOGETHER, int N> __device__ __forceinline__ void add(const float (&x)[N]) {
+    static_assert(N % TOGETHER == 0, "values");
+    const double m = logit_of(top);
+#pragma unroll
+    for (int i = 0; i < N; i += TOGETHER) {
+      double d[TOGETHER];
+#pragma unroll
+      for (int j = 0; j < TOGETHER; ++j) d[j] = __dsub_rn(double(x[i + j]), m);
+      exp_below(d);
+#pragma unroll
+      for (int j = 0; j < TOGETHER; ++j) sum = __dadd_rn(sum, d[j]);
+    }
   }
   __device__ __forceinline__ void join_warp() {
     raise(__reduce_max_sync(kAll, top));
@@ -124,6 +139,18 @@ __device__ __forceinline__ uint64_t sort32(uint64_t v) {
     for (int j = k / 2; j > 0; j /= 2) v = exchange(v, j, ((lane & j) == 0) == ((lane & k) == 0));
   return v;
 }
+// The same of plain keys.
+__device__ __forceinline__ uint32_t sort32_keys(uint32_t v) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int k = 2; k <= 32; k *= 2)
+#pragma unroll
+    for (int j = k / 2; j > 0; j /= 2) {
+      const uint32_t o = __shfl_xor_sync(kAll, v, j);
+      v = ((lane & j) == 0) == ((lane & k) == 0) ? max(v, o) : min(v, o);
+    }
+  return v;
+}
 // The best 32 of two sorted lists, sorted.
 __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b) {
   const int lane = threadIdx.x % 32;
@@ -139,6 +166,7 @@ struct Best {
   uint64_t mine = 0; // the lane-th best
   uint64_t bar = 0;  // only entries above it can still matter
   int held = 0;      // entries waiting in the warp's kWaiting places
+  bool any = false;  // mine is not empty
   __device__ __forceinline__ void flush(uint64_t *wait, int beams) {
     const int lane = threadIdx.x % 32;
     __syncwarp();
@@ -147,7 +175,8 @@ struct Best {
     wait[lane] = later;
     __syncwarp();
     held = max(held - 32, 0);
-    mine = merge32(mine, sort32(v));
+    mine = any ? merge32(mine, sort32(v)) : sort32(v);
+    any = true;
     const uint64_t last = __shfl_sync(kAll, mine, beams - 1);
     bar = bar > last ? bar : last;
   }
@@ -163,7 +192,7 @@ struct Best {
 // Streams over tokens [v0, v1) of a row.  kStep values a lane are in flight;
 // nine cover the byte vocabulary (264) in one step.
 constexpr int kStep = 9;
-template <class T>
+template <class T, int TOGETHER>
 __device__ __forceinline__ void stream_row(const BeamArgs &a, const T *x, int v0, int v1, LogSum &ls, Best &best,
                                            uint64_t *wait) {
   const int lane = threadIdx.x % 32;
@@ -174,30 +203,37 @@ __device__ __forceinline__ void stream_row(const BeamArgs &a, const T *x, int v0
   };
   if (v0 < v1) load(v0);
   for (int v = v0; v < v1; v += 32 * kStep) {
+    float logit[kStep];
     uint32_t key[kStep], top = 0;
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) key[i] = v + 32 * i + lane < v1 ? key_of(to_f32<T>(next[i])) : 0u;
     if (a.allowed) {
       uint8_t ok[kStep];
 #pragma unroll
       for (int i = 0; i < kStep; ++i) ok[i] = a.allowed[min(v + 32 * i + lane, v1 - 1)];
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) key[i] = ok[i] ? key[i] : 0u;
+      for (int i = 0; i < kStep; ++i) logit[i] = ok[i] && v + 32 * i + lane < v1 ? to_f32<T>(next[i]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) logit[i] = v + 32 * i + lane < v1 ? to_f32<T>(next[i]) : -INFINITY;
     }
     if (v + 32 * kStep < v1) load(v + 32 * kStep);
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) top = max(top, key[i]);
+    for (int i = 0; i < kStep; ++i) key[i] = key_of(logit[i]), top = max(top, key[i]);
     if (top > ls.top) ls.raise(top);
-    double term[kStep];
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) term[i] = ls.term(key[i]);
-#pragma unroll
-    for (int i = 0; i < kStep; ++i) ls.sum = __dadd_rn(ls.sum, term[i]);
+    ls.add<TOGETHER>(logit);
     if (v == v0) // of the lanes' largest, the beams-th: at least `beams` values reach it
-      best.bar = uint64_t(entry_key(__shfl_sync(kAll, sort32(uint64_t(top) << 32), a.beams - 1))) << 32;
-    if (!__any_sync(kAll, top >= entry_key(best.bar) && top)) continue;
+      best.bar = uint64_t(__shfl_sync(kAll, sort32_keys(top), a.beams - 1)) << 32;
+    // A lane's values that may matter, one a round: few do.
+    uint32_t some = 0;
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) best.push(entry(key[i], v + 32 * i + lane), wait, a.beams);
+    for (int i = 0; i < kStep; ++i) some |= uint32_t(key[i] && key[i] >= entry_key(best.bar)) << i;
+    while (__any_sync(kAll, some != 0)) {
+      const int which = __ffs(some) - 1;
+      uint32_t k = 0;
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) k = i == which ? key[i] : k;
+      best.push(entry(k, v + 32 * which + lane), wait, a.beams);
+      some &= some - 1;
+    }
   }
   while (best.held) best.flush(wait, a.beams);
 }
@@ -253,8 +289,11 @@ struct Beam {
 };
 
 // A group's results from its beams' best logits; warp w is beam w, lane its
-// place in the list.  Every warp's entries leave its share of shared memory,
-// whose lists are then merged in pairs; the first warp's is the answer.
+// place in the list.  Up to kCountBeams beams: every candidate counts those
+// before it (W^3 / 32 comparisons a lane).  More: the lists are merged in pairs
+// and the first warp's is the answer.  (8 beams: counting @C8@ clocks, merging
+// 2,750; 32 beams: merging 6,500.)
+constexpr int kCountBeams = 16;
 __device__ __forceinline__ void finish_group(const BeamArgs &a, int group, const Beam &beam, const LogSum &ls,
                                              uint64_t mine, WarpShare *shares) {
   const int lane = threadIdx.x % 32, w = threadIdx.x / 32, W = a.beams;
@@ -262,7 +301,7 @@ __device__ __forceinline__ void finish_group(const BeamArgs &a, int group, const
   int token = a.pad;
   if (beam.exists && beam.finished) {
     if (lane == 0) c.key = key_of_total(double(beam.score));
-  } else if (beam.exists && ls.top != 0 && ls.top != kBadKey) {
+  } else if (beam.exists && ls.top != 0 && ls.top < kBadKey) {
     const double lse = __dadd_rn(double(logit_of(ls.top)), log(ls.sum));
     token = entry_token(mine);
     if (lane < W && mine) c.key = key_of_total(__dadd_rn(double(beam.score), __dsub_rn(double(logit_of(entry_key(mine))), lse)));
@@ -273,6 +312,40 @@ __device__ __forceinline__ void finish_group(const BeamArgs &a, int group, const
   list.token[lane] = token;
   int *done = reinterpret_cast<int *>(shares + W); // of each beam
   if (lane == 0) done[w] = beam.finished;
+  const auto write = [&](int slot, const Cand &best) {
+    const long at = long(group) * W + slot;
+    if (best.key) {
+      const int parent = best.id / 32, chosen = shares[parent].list.token[best.id % 32];
+      a.next_scores[at] = float(total_of(best.key));
+      a.tokens[at] = chosen;
+      a.parents[at] = parent;
+      a.next_finished[at] = done[parent] || chosen == a.end;
+    } else { // no candidate fills this slot
+      a.next_scores[at] = -INFINITY;
+      a.tokens[at] = a.pad;
+      a.parents[at] = slot;
+      a.next_finished[at] = 1;
+    }
+  };
+  if (W <= kCountBeams) {
+    // A candidate's slot is the number of candidates before it.  Each of the
+    // warp's W is counted by 32 / P lanes.
+    list.key[lane] = c.key;
+    __syncthreads();
+    const int P = W <= 1 ? 1 : 1 << (32 - __clz(W - 1)), p = lane % P;
+    const uint64_t key = list.key[p];
+    int rank = 0, empty = 0;
+    for (int i = lane / P; i < W * W; i += 32 / P) {
+      const int o = i / W;
+      const uint64_t other = shares[o].list.key[i - o * W];
+      rank += other > key || (other == key && i < w * W + p);
+      empty += other == 0;
+    }
+    for (int o = 16; o >= P; o /= 2) rank += __shfl_xor_sync(kAll, rank, o), empty += __shfl_xor_sync(kAll, empty, o);
+    if (lane < W && key && rank < W) write(rank, {key, uint32_t(w * 32 + lane)});
+    if (w == 0 && lane < W && lane >= W * W - empty) write(lane, Cand());
+    return;
+  }
   for (int step = 1; step < W; step *= 2) {
     if (w % (2 * step) == step) list.key[lane] = c.key, list.id[lane] = c.id;
     __syncthreads();
@@ -281,25 +354,12 @@ __device__ __forceinline__ void finish_group(const BeamArgs &a, int group, const
       c = merge_cands(c, {other.key[lane], other.id[lane]});
     }
   }
-  if (w || lane >= W) return;
-  const long at = long(group) * W + lane;
-  if (c.key) {
-    const int parent = c.id / 32, chosen = shares[parent].list.token[c.id % 32];
-    a.next_scores[at] = float(total_of(c.key));
-    a.tokens[at] = chosen;
-    a.parents[at] = parent;
-    a.next_finished[at] = done[parent] || chosen == a.end;
-  } else { // no candidate fills this slot
-    a.next_scores[at] = -INFINITY;
-    a.tokens[at] = a.pad;
-    a.parents[at] = lane;
-    a.next_finished[at] = 1;
-  }
+  if (w == 0 && lane < W) write(lane, c);
 }
 size_t share_bytes(int beams) { return beams * (sizeof(WarpShare) + sizeof(int)); }
 
 // One launch: one CTA a group, one warp a beam.
-template <class T> __global__ void __launch_bounds__(1024) k_beam_rows(BeamArgs a) {
+template <class T, int THREADS> __global__ void __launch_bounds__(THREADS) k_beam_rows(BeamArgs a) {
   extern __shared__ uint64_t shared[];
   WarpShare *shares = reinterpret_cast<WarpShare *>(shared);
   const int w = threadIdx.x / 32;
@@ -308,7 +368,8 @@ template <class T> __global__ void __launch_bounds__(1024) k_beam_rows(BeamArgs 
   LogSum ls;
   Best best;
   if (beam.exists && !beam.finished) {
-    stream_row<T>(a, static_cast<const T *>(a.logits) + row * a.ld, 0, a.vocab, ls, best, shares[w].wait);
+    stream_row<T, THREADS == 512 ? 9 : 3>(a, static_cast<const T *>(a.logits) + row * a.ld, 0, a.vocab, ls, best,
+                                          shares[w].wait);
     ls.join_warp();
   }
   finish_group(a, blockIdx.x, beam, ls, best.mine, shares);
@@ -328,14 +389,17 @@ struct Slice {
 
 // One launch serves short rows, and rows enough to give every SM eight warps.
 __host__ __device__ inline bool in_slices(long rows, int vocab) { return vocab > kRowsVocab && rows < kManyRows; }
-// Slices of a row: about four CTAs an SM, none shorter than a warp's step of values for every warp.
+constexpr int kStepValues = 32 * kStep;
+__host__ __device__ inline int row_steps(int vocab) { return (vocab + kStepValues - 1) / kStepValues; }
+// Slices of a row: so many steps a warp that all CTAs run at once (three an
+// SM), and no more slices than these steps fill.
 __host__ __device__ inline int slice_count(long rows, int vocab) {
-  const int want = int((4 * 148 + rows - 1) / rows), most = (vocab + 32 * kStep * kSliceWarps - 1) / (32 * kStep * kSliceWarps);
-  const int n = want < most ? want : most;
-  return n < kSlices ? n : kSlices;
+  const int most = rows < 3 * 148 ? int(3 * 148 / rows) : 1, steps = row_steps(vocab);
+  const int slots = (most < kSlices ? most : kSlices) * kSliceWarps, each = (steps + slots - 1) / slots;
+  return (steps + each * kSliceWarps - 1) / (each * kSliceWarps);
 }
 
-template <class T> __global__ void __launch_bounds__(32 * kSliceWarps) k_beam_slice(BeamArgs a, int slices) {
+template <class T> __global__ void __launch_bounds__(32 * kSliceWarps, 3) k_beam_slice(BeamArgs a, int slices) {
   __shared__ uint64_t wait[kSliceWarps][kWaiting];
   __shared__ double sums[kSliceWarps];
   __shared__ uint32_t tops[kSliceWarps];
@@ -344,18 +408,20 @@ template <class T> __global__ void __launch_bounds__(32 * kSliceWarps) k_beam_sl
   const int slice = blockIdx.x % slices;
   const Beam beam(a, row);
   if (!beam.exists || beam.finished) return; // the row's logits do not count
-  const int part = slice * kSliceWarps + warp, parts = slices * kSliceWarps;
+  // Whole steps to every warp.
+  const long part = slice * kSliceWarps + warp, parts = slices * kSliceWarps, steps = row_steps(a.vocab);
   LogSum ls;
   Best best;
-  stream_row<T>(a, static_cast<const T *>(a.logits) + row * a.ld, int(long(part) * a.vocab / parts),
-                int(long(part + 1) * a.vocab / parts), ls, best, wait[warp]);
+  stream_row<T, 9>(a, static_cast<const T *>(a.logits) + row * a.ld, int(min(long(a.vocab), part * steps / parts * kStepValues)),
+                   int(min(long(a.vocab), (part + 1) * steps / parts * kStepValues)), ls, best, wait[warp]);
   ls.join_warp();
-  __syncwarp();
-  wait[warp][lane] = best.mine;
   if (lane == 0) sums[warp] = ls.sum, tops[warp] = ls.top;
-  __syncthreads();
+  for (int step = 1; step < kSliceWarps; step *= 2) { // the warps' lists, in pairs
+    if (warp % (2 * step) == step) wait[warp][lane] = best.mine;
+    __syncthreads();
+    if (warp % (2 * step) == 0) best.mine = merge32(best.mine, wait[warp + step][lane]);
+  }
   if (warp) return;
-  for (int i = 1; i < kSliceWarps; ++i) best.mine = merge32(best.mine, wait[i][lane]);
   LogSum all;
   if (lane < kSliceWarps) all.sum = sums[lane], all.top = tops[lane];
   all.join_warp();
@@ -375,13 +441,18 @@ __global__ void __launch_bounds__(1024) k_beam_join(BeamArgs a, int slices) {
     const Slice *s = static_cast<const Slice *>(a.work) + row * slices;
     if (lane < slices) ls.top = s[lane].top, ls.sum = s[lane].sum;
     ls.join_warp();
-    for (int i = 0; i < slices; i += 4) { // four lists' loads in flight together
+    // The slices' entries one after the other, 32 at a time, four loads in flight.
+    const int entries = slices * a.beams;
+    for (int i = 0; i < entries; i += 128) {
       uint64_t e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) e[j] = i + j < slices && lane < a.beams ? s[i + j].best[lane] : 0;
+      for (int j = 0; j < 4; ++j) {
+        const int at = i + 32 * j + lane, slice = at / a.beams;
+        e[j] = at < entries ? s[slice].best[at - slice * a.beams] : 0;
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (i + j < slices) mine = merge32(mine, e[j]);
+        if (i + 32 * j < entries) mine = i + j ? merge32(mine, sort32(e[j])) : sort32(e[j]);
     }
   }
   finish_group(a, blockIdx.x, beam, ls, mine, reinterpret_cast<WarpShare *>(shared));
@@ -394,7 +465,11 @@ template <class T> void select_typed(const BeamArgs &a, cudaStream_t s) {
     k_beam_slice<T><<<unsigned(rows * slices), 32 * kSliceWarps, 0, s>>>(a, slices);
     k_beam_join<<<a.groups, 32 * a.beams, share_bytes(a.beams), s>>>(a, slices);
   } else {
-    k_beam_rows<T><<<a.groups, 32 * a.beams, share_bytes(a.beams), s>>>(a);
+    // Up to 16 beams leave a thread the registers to keep its values of a step.
+    if (a.beams <= 16)
+      k_beam_rows<T, 512><<<a.groups, 32 * a.beams, share_bytes(a.beams), s>>>(a);
+    else
+      k_beam_rows<T, 1024><<<a.groups, 32 * a.beams, share_bytes(a.beams), s>>>(a);
   }
 }
 
