@@ -20,7 +20,7 @@
 // one a lane; values above the last that matters gather in shared memory and
 // are sorted and merged in 32 at a time, so that most values cost a comparison.
 // (Taking the best out one by one with warp-wide maxima cost 120 instructions
-// a beam and row: 256 x 8 x 264 12.2 us, @SEL_US@ now.)
+// a beam and row: 64 x 32 x 264 38 us, 15.8 now.)
 #include "beam_kernels.h"
 
 #include <cuda_bf16.h>
@@ -62,25 +62,34 @@ __device__ __forceinline__ double warp_sum(double v) {
 // exp of N values <= 0, each to about 1e-12 of it: 2^n times the Taylor
 // polynomial of degree 10 on |r| <= ln 2 / 2 (its remainder is below 3e-13).
 // Below -80, and for a NaN, it is 0: against a sum of at least 1 such a term
-// has no bit.  The values go through each step together: a 64-bit operation
-// takes 8 clocks and another can start every second.
+// has no bit.  The values go through each step together, which the volatile
+// statements keep (9 values of a warp: 916 clocks; one after the other, as the
+// compiler orders plain code, 1,492).
+__constant__ double kTaylor[11] = {1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120,
+                                   1.0 / 24,      1.0 / 6,      0.5,         1.0,        1.0};
+__constant__ double kExp[3] = {6755399441055744.0, // 1.5 * 2^52: the sum's low word is the nearest integer
+                               1.4426950408889634, 0.6931471805599453};
+__device__ __forceinline__ double step_fma(double a, double b, double c) {
+  double r;
+  asm volatile("fma.rn.f64 %0, %1, %2, %3;" : "=d"(r) : "d"(a), "d"(b), "d"(c));
+  return r;
+}
 template <int N> __device__ __forceinline__ void exp_below(double (&v)[N]) {
-  constexpr double kShift = 6755399441055744.0; // 1.5 * 2^52: the sum's low word is the nearest integer
-  constexpr double kTaylor[10] = {1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120,
-                                  1.0 / 24,     1.0 / 6,     0.5,        1.0,       1.0};
   double t[N], p[N];
   bool counts[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     counts[i] = v[i] >= -80.0;
-    t[i] = __fma_rn(v[i], 1.4426950408889634, kShift);
+    t[i] = step_fma(v[i], kExp[1], kExp[0]);
   }
 #pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = __fma_rn(-__dsub_rn(t[i], kShift), 0.6931471805599453, v[i]), p[i] = 1.0 / 3628800;
+  for (int i = 0; i < N; ++i) v[i] = step_fma(-__dsub_rn(t[i], kExp[0]), kExp[2], v[i]);
 #pragma unroll
-  for (int k = 0; k < 10; ++k)
+  for (int i = 0; i < N; ++i) p[i] = step_fma(v[i], kTaylor[0], kTaylor[1]);
 #pragma unroll
-    for (int i = 0; i < N; ++i) p[i] = __fma_rn(p[i], v[i], kTaylor[k]);
+  for (int k = 2; k < 11; ++k)
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = step_fma(p[i], v[i], kTaylor[k]);
 #pragma unroll
   for (int i = 0; i < N; ++i)
     v[i] = counts[i] ? __hiloint2double(__double2hiint(p[i]) + (__double2loint(t[i]) << 20), __double2loint(p[i])) : 0.0;
@@ -291,8 +300,8 @@ struct Beam {
 // A group's results from its beams' best logits; warp w is beam w, lane its
 // place in the list.  Up to kCountBeams beams: every candidate counts those
 // before it (W^3 / 32 comparisons a lane).  More: the lists are merged in pairs
-// and the first warp's is the answer.  (8 beams: counting @C8@ clocks, merging
-// 2,750; 32 beams: merging 6,500.)
+// and the first warp's is the answer.  (4 beams: counting 1,090 clocks,
+// merging 1,860; 8 beams: 2,450, 2,750; 32 beams: merging 6,500.)
 constexpr int kCountBeams = 16;
 __device__ __forceinline__ void finish_group(const BeamArgs &a, int group, const Beam &beam, const LogSum &ls,
                                              uint64_t mine, WarpShare *shares) {
@@ -473,43 +482,61 @@ template <class T> void select_typed(const BeamArgs &a, cudaStream_t s) {
   }
 }
 
-// Reordering: a thread owns one unit (16, 4, 2 or 1 bytes) of the columns of
-// one group's rows.  It reads that unit of every row that moves before it
-// writes any, and no other thread touches these columns: the rows can be
-// permuted, and copied to several places, in place and in one pass.
-constexpr int kMoveThreads = 256;
-
-template <class U, int W> __global__ void __launch_bounds__(kMoveThreads) k_state_reorder(ReorderArgs a, long units) {
+// Reordering: a thread owns U units (of 16, 4, 2 or 1 bytes) of the columns of
+// one group's rows.  It reads them of every row that moves before it writes
+// any, and no other thread touches these columns: the rows can be permuted, and
+// copied to several places, in place and in one pass.  U makes up for few
+// beams: about 16 units in flight a thread (2048 x 2 x 11008: one unit 45 us,
+// four 31; 256 x 8 x 44032: one 86 us, two 78, the copy rate).
+template <class T, int W, int U> __global__ void __launch_bounds__(W == 32 ? 128 : 256) k_state_reorder(ReorderArgs a, long units) {
   __shared__ int from[kMaxBeams];
-  const long chunks = (units + kMoveThreads - 1) / kMoveThreads;
-  const long group = blockIdx.x / chunks, u = blockIdx.x % chunks * kMoveThreads + threadIdx.x;
+  constexpr int kMoveThreads = W == 32 ? 128 : 256; // 32 rows: three small CTAs an SM, so that loads and stores overlap
+  constexpr int kSpan = kMoveThreads * U;
+  const long chunks = (units + kSpan - 1) / kSpan;
+  const long group = blockIdx.x / chunks, u0 = blockIdx.x % chunks * kSpan + threadIdx.x;
   if (threadIdx.x < a.beams) {
     const int p = a.parents[group * a.beams + threadIdx.x];
     from[threadIdx.x] = p >= 0 && p < a.beams ? p : int(threadIdx.x);
   }
   __syncthreads();
-  if (u >= units) return;
-  char *base = static_cast<char *>(a.states) + group * a.beams * a.ld_bytes + u * long(sizeof(U));
-  U v[W];
+  char *base = static_cast<char *>(a.states) + group * a.beams * a.ld_bytes + u0 * long(sizeof(T));
+  T v[W][U];
 #pragma unroll
-  for (int w = 0; w < W; ++w)
-    if (w < a.beams && from[w] != w) v[w] = *reinterpret_cast<const U *>(base + from[w] * a.ld_bytes);
+  for (int w = 0; w < W; ++w) {
+    if (w >= a.beams || from[w] == w) continue;
+    const char *row = base + from[w] * a.ld_bytes;
 #pragma unroll
-  for (int w = 0; w < W; ++w)
-    if (w < a.beams && from[w] != w) *reinterpret_cast<U *>(base + w * a.ld_bytes) = v[w];
+    for (int i = 0; i < U; ++i)
+      if (u0 + i * kMoveThreads < units) v[w][i] = *reinterpret_cast<const T *>(row + i * kMoveThreads * sizeof(T));
+  }
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    if (w >= a.beams || from[w] == w) continue;
+    char *row = base + w * a.ld_bytes;
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (u0 + i * kMoveThreads < units) *reinterpret_cast<T *>(row + i * kMoveThreads * sizeof(T)) = v[w][i];
+  }
 }
 
-template <class U> void reorder_unit(const ReorderArgs &a, cudaStream_t s) {
-  const long units = a.row_bytes / long(sizeof(U)), blocks = (units + kMoveThreads - 1) / kMoveThreads * a.groups;
+template <class T, int W, int U> void reorder_launch(const ReorderArgs &a, cudaStream_t s) {
+  constexpr int kMoveThreads = W == 32 ? 128 : 256;
+  const long units = a.row_bytes / long(sizeof(T)), blocks = (units + kMoveThreads * U - 1) / (kMoveThreads * U) * a.groups;
   if (blocks > 0x7FFFFFFFL) throw std::invalid_argument("Too many states to reorder in one call");
-  if (a.beams <= 4)
-    k_state_reorder<U, 4><<<unsigned(blocks), kMoveThreads, 0, s>>>(a, units);
+  k_state_reorder<T, W, U><<<unsigned(blocks), kMoveThreads, 0, s>>>(a, units);
+}
+
+template <class T> void reorder_unit(const ReorderArgs &a, cudaStream_t s) {
+  if (a.beams <= 2)
+    reorder_launch<T, 2, 8>(a, s);
+  else if (a.beams <= 4)
+    reorder_launch<T, 4, 4>(a, s);
   else if (a.beams <= 8)
-    k_state_reorder<U, 8><<<unsigned(blocks), kMoveThreads, 0, s>>>(a, units);
+    reorder_launch<T, 8, 2>(a, s);
   else if (a.beams <= 16)
-    k_state_reorder<U, 16><<<unsigned(blocks), kMoveThreads, 0, s>>>(a, units);
+    reorder_launch<T, 16, 1>(a, s);
   else
-    k_state_reorder<U, 32><<<unsigned(blocks), kMoveThreads, 0, s>>>(a, units);
+    reorder_launch<T, 32, 1>(a, s);
 }
 
 } // namespace
