@@ -388,7 +388,6 @@ template <class T, int THREADS> __global__ void __launch_bounds__(THREADS) k_bea
 // to kSlices slices, one CTA a slice; a slice leaves its sum and its sorted
 // best entries in the workspace, and one CTA a group joins them.
 constexpr int kSliceWarps = 8, kSlices = 32;
-constexpr int kRowsVocab = 2048, kManyRows = 1184; // see in_slices
 
 struct Slice {
   double sum;
@@ -396,8 +395,13 @@ struct Slice {
   uint64_t best[kMaxBeams];
 };
 
-// One launch serves short rows, and rows enough to give every SM eight warps.
-__host__ __device__ inline bool in_slices(long rows, int vocab) { return vocab > kRowsVocab && rows < kManyRows; }
+// One launch serves short rows, and rows enough to give every SM eight warps
+// (one launch / two: 64 rows x 512 8.3 / 12.4 us, x 2000 14.4 / 11.3; 512 rows
+// x 2000 16.4 / 18.5, x 5000 31 / 25; 1024 rows x 20000 89 / 66; 2048 rows x
+// 5000 39 / 53, x 20000 115 / 121).
+__host__ __device__ inline bool in_slices(long rows, int vocab) {
+  return rows < 8 * 148 && vocab > (rows < 256 ? 1024 : 2048);
+}
 constexpr int kStepValues = 32 * kStep;
 __host__ __device__ inline int row_steps(int vocab) { return (vocab + kStepValues - 1) / kStepValues; }
 // Slices of a row: so many steps a warp that all CTAs run at once (three an
