@@ -351,11 +351,14 @@ int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale
  * next_scores, tokens, parents (the beam within the group) and next_finished
  * (the parent's, or the token is `end`; end < 0: no token ends a beam).  Scores
  * are formed in 64 bits and rounded once; a beam's equal logits go to the lower
- * token, equal scores of two beams to the lower beam.  A candidate whose score
+ * token, equal 64-bit scores of two beams to the lower beam (rows that hold the
+ * same values in another order have sums that may differ in their last bits).
+ * A candidate whose score
  * is not finite is none (a row whose mask leaves nothing, or that holds a NaN
  * or +inf at an allowed token, has none); slots that no candidate fills get
  * score -inf, `pad`, their own index as parent, and count as finished.
- * next_scores may be scores and next_finished may be finished. */
+ * next_scores may be scores and next_finished may be finished.  The workspace
+ * (ng_beam_workspace bytes, 0 for many sizes) belongs to one call at a time. */
 size_t ng_beam_workspace(int groups, int beams, int vocab);
 int ng_beam_select(int device, const void *logits, int dtype, int64_t ld, int groups, int beams, int vocab,
                    const float *scores, const uint8_t *finished, const uint8_t *allowed, int end, int pad,

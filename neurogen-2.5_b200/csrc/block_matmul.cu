@@ -485,7 +485,7 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
     const uint32_t from = tmem + (uint32_t(warp % 4 * 32) << 16) + group * S::kCols;
     uint64_t sum[S::kCols / 2];
     uint32_t d[2][32];
-    bool alive = !stalled;
+    bool alive = !stalled, met = false; // met: the cluster's CTAs are known to run
     const int sets = (kb1 - kb0 + S::kPair - 1) / S::kPair;                       // of accumulators a tile
     int left = first < tiles ? ((tiles - 1 - first) / stride + 1) * sets : 0; // still to add
     int acc = 0, chunk = 0; // set in turn, scale buffers taken so far
@@ -544,6 +544,7 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
         store_rows<Y, S::kCols>(a, m0, n0, sum, vec, swap + warp * 128);
       } else {
         cluster_wait();
+        met = true;
         const int rows = kTileM / splits, owner = row / rows;
         float4 *to = cg::this_cluster().map_shared_rank(part, owner) + long(z) * (S::kCols / 4) * (rows + 1) + row % rows;
 #pragma unroll
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
         }
       }
     }
-    if (splits > 1 && !alive) cluster_wait();
+    if (splits > 1 && !met) cluster_wait();
   } else {
     if constexpr (S::kGroups == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFewerRegs));
     // The copies' and MMAs' warps run as one and elect the lane that issues:

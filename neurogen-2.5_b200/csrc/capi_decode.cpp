@@ -78,7 +78,7 @@ int ng_block_quantize(int device, const void *x, int dtype, int64_t rows, int64_
     QuantArgs a{};
     a.type = elem(dtype);
     require(block_rows == 1 || block_rows == kScaleBlock, "A scale covers 1 or 128 rows");
-    require(rows >= 0 && rows <= INT_MAX && cols >= 1 && cols <= INT_MAX, "Matrix size out of range");
+    require(rows >= 0 && rows <= INT_MAX && cols >= 1 && cols <= INT_MAX / 2, "Matrix size out of range");
     require(ldx >= cols && ldq >= cols, "Row stride smaller than the row");
     const int64_t blocks = blocks_of(rows, block_rows) * blocks_of(cols, kScaleBlock);
     require(blocks <= INT_MAX, "Matrix size out of range");

@@ -506,6 +506,12 @@ class SessionPool:
             raise ValueError('Token must be in 0..263')
         if steps < 1:
             raise ValueError('Need at least one step')
+        if end is not None and not 0 <= end < VOCAB:
+            raise ValueError('End token outside the vocabulary')
+        if allowed is not None:
+            allowed = torch.as_tensor(allowed)
+            if allowed.dtype != torch.bool or tuple(allowed.shape) != (VOCAB,):
+                raise ValueError(f'allowed must be bool [{VOCAB}]')
         device = torch.device('cuda', self.lib.ng_pool_device(self.h))
         # A stream of its own: the pool's calls take the default stream's handle, 0, for the engine's stream.
         side = torch.cuda.Stream(device)
@@ -515,7 +521,7 @@ class SessionPool:
             logits = torch.empty((self.sessions, VOCAB), device=device)
             feed = torch.from_numpy(prompts.T.astype(np.int32)).to(device).repeat_interleave(beams, 1)
             if allowed is not None:
-                allowed = torch.as_tensor(allowed).to(device)
+                allowed = allowed.to(device).contiguous()
             first = torch.zeros((groups, beams), dtype=torch.int32, device=device)
             self._check(self.lib.ng_pool_reorder_device(self.h, beams, first.data_ptr(), stream))
 

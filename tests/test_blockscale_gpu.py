@@ -100,6 +100,40 @@ def test_quantize_edges(rows):
     assert np.array_equal(scale.cpu().numpy(), want_scale) and np.array_equal(bytes_of(q), want_q)
 
 
+@pytest.mark.parametrize('dtype', list(TYPES))
+def test_quantize_16_bit_extremes(dtype):
+    """A NaN of either sign, infinities and the type's largest value, in both block shapes."""
+    info = torch.finfo(TYPES[dtype])
+    x = wide_values(3, 130, 260, TYPES[dtype])
+    x[1, 3], x[2, 130], x[129, 259], x[0, 5] = float('nan'), -float('inf'), info.max, -info.max
+    x[3, 200] = torch.tensor(-float('nan'))
+    for rows in (1, 128):
+        for view in (x.cuda(), torch.cat([x[:, :1], x], 1).cuda()[:, 1:]):
+            q, s = blockscale.quantize(view, rows)
+            bad = torch.zeros(130, 260, dtype=torch.bool)
+            bad[1, 3] = bad[2, 130] = bad[3, 200] = True
+            per = bad.float().new_zeros(-(-130 // rows) * rows, 384)
+            per[:130, :260] = bad.float()
+            per = per.view(-1, rows, 3, 128).amax((1, 3)) > 0
+            assert torch.equal(torch.isfinite(s.cpu()), ~per)
+            want_q, want_s = quantize_64(torch.where(bad, 0, x).double().numpy(), rows)
+            ok = ~per.repeat_interleave(rows, 0)[:130].repeat_interleave(128, 1)[:, :260].numpy()
+            assert np.array_equal(bytes_of(q)[ok], want_q[ok])
+            assert np.array_equal(s.cpu().numpy()[~per.numpy()], want_s[~per.numpy()])
+
+
+def test_matmul_far_rows():
+    """A result whose offsets pass 32 bits, against 64 bits at its corners."""
+    m, n, k = 70_000, 40_000, 32
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    a, sa = blockscale.quantize(torch.randn((m, k), generator=gen, device='cuda'))
+    w, sw = blockscale.quantize(torch.randn((n, k), generator=gen, device='cuda'), 128)
+    y = blockscale.matmul(a, sa, w, sw, out_dtype=torch.bfloat16)
+    for rows in (slice(0, 200), slice(35_000, 35_100), slice(m - 130, m)):
+        want, size = product_64(a[rows], sa[rows], w, sw)
+        assert ((y[rows].double() - want).abs() <= (128 + 1 + 4) * 2.0 ** -23 * size + 2.0 ** -8 * want.abs()).all()
+
+
 def test_quantize_non_finite():
     x = wide_values(1, 4, 300, torch.float32)
     x[1, 10] = float('nan')

@@ -27,6 +27,7 @@ def quantize(x=P, dtype=0, rows=4, cols=300, ldx=300, block=1, q=P, ldq=304, sca
     (dict(dtype=3), 'Element type'), (dict(dtype=-1), 'Element type'), (dict(block=2), '1 or 128 rows'),
     (dict(rows=-1), 'out of range'), (dict(cols=0), 'out of range'), (dict(rows=1 << 31), 'out of range'),
     (dict(rows=(1 << 31) - 1, cols=1 << 20, ldx=1 << 20, ldq=1 << 20), 'out of range'),
+    (dict(rows=1, cols=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31), 'out of range'),
     (dict(ldx=299), 'Row stride'), (dict(ldq=288), 'Row stride'), (dict(ldq=308), '16-byte'),
     (dict(q=P + 8), '16-byte'), (dict(x=None), 'Null'), (dict(q=None), 'Null'), (dict(scale=None), 'Null'),
     (dict(x=P + 2), 'aligned'), (dict(x=P + 1, dtype=1), 'aligned'), (dict(scale=P + 2), 'aligned'),
@@ -60,7 +61,7 @@ def select(logits=P, dtype=0, ld=264, groups=2, beams=4, vocab=264, scores=P, en
 
 @pytest.mark.parametrize('change,text', [
     (dict(dtype=3), 'Element type'), (dict(beams=0), '1..32'), (dict(beams=33), '1..32'),
-    (dict(vocab=0), 'Vocabulary'), (dict(groups=-1), 'Too many'), (dict(groups=1 << 28, beams=32), 'Too many'),
+    (dict(vocab=0), 'Vocabulary'), (dict(vocab=(1 << 30) + 1, ld=1 << 31), 'Vocabulary'), (dict(groups=-1), 'Too many'), (dict(groups=1 << 28, beams=32), 'Too many'),
     (dict(ld=263), 'Row stride'), (dict(pad=264), 'Padding token'), (dict(pad=-1), 'Padding token'),
     (dict(end=264), 'End token'), (dict(logits=None), 'Null'), (dict(scores=None), 'Null'), (dict(out=None), 'Null'),
     (dict(logits=P + 2), 'aligned'), (dict(scores=P + 2), 'aligned'),

@@ -95,6 +95,39 @@ def test_select(groups, beams, dtype, vocab):
     check_select(logits, scores, finished, allowed, end=int(rng.integers(vocab)), pad=int(rng.integers(vocab)))
 
 
+@pytest.mark.parametrize('groups,beams,vocab,dtype', [(400, 3, 3000, 'bf16'), (1300, 1, 2500, 'fp32'), (40, 32, 2100, 'fp16'),
+                                                      (70, 16, 1200, 'fp32'), (3, 17, 1500, 'fp32'), (130, 2, 5000, 'fp32')])
+def test_select_either_side_of_the_two_launch_rule(groups, beams, vocab, dtype):
+    """Long rows by one launch (many rows) and by two (few)."""
+    rng, logits, scores = inputs(vocab + groups, groups, beams, vocab, TYPES[dtype])
+    finished = torch.from_numpy(rng.random((groups, beams)) < 0.2)
+    allowed = torch.from_numpy(rng.random(vocab) < 0.9)
+    check_select(logits, scores, finished, allowed, end=7)
+
+
+def test_select_ascending_and_descending_rows():
+    """Orders that fill the held-back entries most often: every value above all before it, and none.
+    Within a call all rows have one order: a row and its reverse have the same score as real numbers,
+    and a 64-bit sum of `vocab` terms, off by up to vocab 2^-53, puts either first."""
+    for beams in (1, 6, 32):
+        for vocab in (264, 1000, 5000):
+            row = torch.arange(vocab).float() / 64
+            for order in (row, row.flip(0)):
+                logits = order.expand(2 * beams, vocab).contiguous()
+                check_select(logits, torch.zeros(2, beams))
+                check_select((logits * 2).round(), torch.zeros(2, beams))
+
+
+def test_select_far_rows():
+    """Rows whose offsets pass 32 bits."""
+    ld = 40_000_000
+    big = torch.empty(64 * ld, dtype=torch.bfloat16, device='cuda').view(64, ld)
+    for vocab in (300, 3000):
+        rng, logits, scores = inputs(1, 16, 4, vocab, torch.bfloat16)
+        big[:, 3:3 + vocab] = logits.cuda()
+        check_select(big[:, 3:3 + vocab], scores)
+
+
 @pytest.mark.parametrize('vocab', [40, 264, 900, 3000, 9000])
 def test_select_ties_go_to_the_lower_index(vocab):
     """Equal logits within a beam, equal beams, and both; a vocabulary of one value only."""
@@ -187,7 +220,8 @@ def reorder_plain(states, parents):
 
 @pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.uint8, torch.float64])
 @pytest.mark.parametrize('groups,beams,size', [(1, 1, 5), (3, 2, 1), (2, 4, 704), (1, 5, 37), (7, 8, 1023), (2, 9, 260),
-                                               (3, 16, 513), (2, 17, 4096), (5, 32, 333)])
+                                               (3, 16, 513), (2, 17, 4096), (5, 32, 333), (2, 2, 9001), (3, 4, 20000),
+                                               (2, 8, 12000), (300, 3, 64)])
 def test_reorder(groups, beams, size, dtype):
     rng = np.random.default_rng(size)
     states = torch.from_numpy(rng.integers(0, 200, (groups * beams + 2, size))).to(dtype)
@@ -199,6 +233,18 @@ def test_reorder(groups, beams, size, dtype):
         assert got.data_ptr() == device.data_ptr()
         assert torch.equal(device[:groups * beams].cpu(), reorder_plain(states[:groups * beams], parents))
         assert torch.equal(device[groups * beams:].cpu(), states[groups * beams:])   # rows behind the last group
+
+
+def test_reorder_far_rows():
+    """Rows whose offsets pass 32 bits."""
+    n = 1_500_000_016
+    states = torch.zeros((3, n), dtype=torch.uint8, device='cuda')
+    at = torch.tensor([0, 1, 77_777, n // 2, n - 2, n - 1], device='cuda')
+    for w in range(3):
+        states[w, at] = torch.arange(6, dtype=torch.uint8, device='cuda') + 10 * w + 1
+    decoding.reorder(states, torch.tensor([[2, 0, 0]], dtype=torch.int32, device='cuda'))
+    assert states[:, at].cpu().tolist() == [[21 + i for i in range(6)], [1 + i for i in range(6)], [1 + i for i in range(6)]]
+    assert states[0].sum(dtype=torch.int64).item() == sum(21 + i for i in range(6))
 
 
 def test_reorder_strided_and_shaped():
@@ -345,8 +391,12 @@ def test_beam_search_equals_a_host_search(groups, beams, steps):
 
 def test_beam_search_refusals():
     pool = SessionPool(pool_model(), 6)
-    for args, text in (((np.zeros((2, 3)), 4, 2), 'divide'), ((np.zeros((2, 3)), 0, 2), 'divide'),
+    before = pool.states()
+    for args, text in (((np.zeros((2, 3)), 3, 2, 264), 'End token'), ((np.zeros((2, 3)), 3, 2, None, np.ones(263, bool)), 'allowed'),
+                       ((np.zeros((2, 3)), 3, 2, None, np.ones(264, np.int32)), 'allowed'),
+                       ((np.zeros((2, 3)), 4, 2), 'divide'), ((np.zeros((2, 3)), 0, 2), 'divide'),
                        ((np.zeros((1, 3)), 3, 2), 'prompts'), ((np.zeros((2, 0)), 3, 2), 'prompts'),
                        ((np.full((2, 3), 264), 3, 2), '0..263'), ((np.zeros((2, 3)), 3, 0), 'one step')):
         with pytest.raises(ValueError, match=text):
             pool.beam_search(*args)
+    assert np.array_equal(pool.states(), before)
