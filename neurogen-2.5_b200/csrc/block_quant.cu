@@ -42,23 +42,24 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
 }
 
 // fl(x / scale) for a whole block by one reciprocal and exact remainders
-// (Markstein): with hi + lo = 1 / scale to 2^-47, q = fl(x hi + fl(x lo)) is a
-// neighbour of the quotient, its remainder is exact, and one step from a
+// (Markstein): with down + lo = 1 / scale to 2^-46, q = fl(x down + fl(x lo)) is
+// a neighbour of the quotient, its remainder is exact, and one step from a
 // neighbour by the rounded reciprocal hi gives the correctly rounded quotient.
 // Four operations a value, where the divisions cost more than the block's
 // bytes (a product that divides only near the ties of e4m3 was no faster: bf16
 // ratios are often short, and most warps had one).  The remainders are exact
 // while scale is at least 2^-90 (a quotient below 2^-11, where they might not
 // be, is the byte 0 in any case) and lo is while it is at most 2^90; other
-// blocks divide.  The signs
-// are such that a zero keeps its own.
+// blocks divide.  down is 1 / scale rounded down and lo not negative, so that
+// both parts of a zero's quotient have its sign; the last step's signs keep it.
 struct BlockScale {
-  float scale, hi, lo;
+  float scale, hi, down, lo;
   bool divide;
   __device__ __forceinline__ explicit BlockScale(uint32_t amax_bits) {
     scale = block_scale(amax_bits);
     hi = __fdiv_rn(1.f, scale);
-    lo = __fmul_rn(__fmaf_rn(-scale, hi, 1.f), hi);
+    down = __fmaf_rn(-scale, hi, 1.f) < 0.f ? __uint_as_float(__float_as_uint(hi) - 1u) : hi;
+    lo = __fmul_rn(__fmaf_rn(-scale, down, 1.f), hi);
     divide = !(scale >= 0x1p-90f && scale <= 0x1p90f);
   }
   __device__ __forceinline__ uint32_t quantize4(const float (&v)[4]) const {
@@ -69,7 +70,7 @@ struct BlockScale {
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        q[i] = __fmaf_rn(v[i], hi, __fmul_rn(v[i], lo));
+        q[i] = __fmaf_rn(v[i], down, __fmul_rn(v[i], lo));
         q[i] = __fmaf_rn(-__fmaf_rn(q[i], scale, -v[i]), hi, q[i]);
       }
     }

@@ -100,6 +100,22 @@ def test_quantize_edges(rows):
     assert np.array_equal(scale.cpu().numpy(), want_scale) and np.array_equal(bytes_of(q), want_q)
 
 
+@pytest.mark.parametrize('rows', [1, 128])
+@pytest.mark.parametrize('dtype', list(TYPES))
+def test_quantize_zeros_and_underflow_keep_their_sign(dtype, rows):
+    """Zeros of either sign, and values whose quotient rounds to zero, next to values of many scales
+    (the reciprocal of a scale may be rounded up or down)."""
+    x = wide_values(5, 130, 128 * 40, TYPES[dtype])
+    x[:, 3::16] = 0.0
+    x[:, 5::16] = -0.0
+    x[:, 7::16] *= 2.0 ** -12
+    x[:, 9::16] *= torch.finfo(TYPES[dtype]).tiny
+    q, scale = blockscale.quantize(x.cuda(), rows)
+    want_q, want_scale = quantize_64(x.double().numpy(), rows)
+    assert np.array_equal(scale.cpu().numpy(), want_scale)
+    assert np.array_equal(bytes_of(q), want_q)
+
+
 @pytest.mark.parametrize('dtype', list(TYPES))
 def test_quantize_16_bit_extremes(dtype):
     """A NaN of either sign, infinities and the type's largest value, in both block shapes."""
