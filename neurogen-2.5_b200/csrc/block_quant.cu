@@ -41,13 +41,35 @@ __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d
   return uint32_t(lo) | (uint32_t(hi) << 16);
 }
 
+// Packed pairs of fp32: each half is one IEEE operation.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float &lo, float &hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 // fl(x / scale) for a whole block by one reciprocal and exact remainders
 // (Markstein): with down + lo = 1 / scale to 2^-46, q = fl(x down + fl(x lo)) is
 // a neighbour of the quotient, its remainder is exact, and one step from a
 // neighbour by the rounded reciprocal hi gives the correctly rounded quotient.
-// Four operations a value, where the divisions cost more than the block's
-// bytes (a product that divides only near the ties of e4m3 was no faster: bf16
-// ratios are often short, and most warps had one).  The remainders are exact
+// Four operations a value, two a packed instruction (8192 x 8192 bf16 40 us,
+// 45 one by one), where the divisions cost more than the block's bytes (a
+// product that divides only near the ties of e4m3 was no faster: bf16 ratios
+// are often short, and most warps had one).  The remainders are exact
 // while scale is at least 2^-90 (a quotient below 2^-11, where they might not
 // be, is the byte 0 in any case) and lo is while it is at most 2^90; other
 // blocks divide.  down is 1 / scale rounded down and lo not negative, so that
@@ -62,19 +84,21 @@ struct BlockScale {
     lo = __fmul_rn(__fmaf_rn(-scale, down, 1.f), hi);
     divide = !(scale >= 0x1p-90f && scale <= 0x1p90f);
   }
+  // Four values, the quotients negated until the last step so that no value
+  // changes sign before; pairs go through one packed instruction a step.
   __device__ __forceinline__ uint32_t quantize4(const float (&v)[4]) const {
     float q[4];
     if (divide) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) q[i] = __fdiv_rn(v[i], scale);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        q[i] = __fmaf_rn(v[i], down, __fmul_rn(v[i], lo));
-        q[i] = __fmaf_rn(-__fmaf_rn(q[i], scale, -v[i]), hi, q[i]);
-      }
+      return pack_e4m3(q[0], q[1], q[2], q[3]);
     }
-    return pack_e4m3(q[0], q[1], q[2], q[3]);
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const f32x2 x = pack2(v[i], v[i + 1]), n = fma2(x, pack2(-down, -down), mul2(x, pack2(-lo, -lo)));
+      unpack2(fma2(fma2(n, pack2(scale, scale), x), pack2(-hi, -hi), n), q[i], q[i + 1]);
+    }
+    return pack_e4m3(q[0], q[1], q[2], q[3]) ^ 0x80808080u;
   }
 };
 
@@ -82,8 +106,11 @@ struct BlockScale {
 // VEC: the row's start and stride allow one load.  Otherwise four loads of 32
 // bits, or for 16-bit types the one or two aligned 16-byte words that hold
 // them, shifted into place; a word with one byte of the row lies within the
-// row's memory (8000 x 8100 bf16, 128 x 128 blocks: 61 us, with a load a value
-// 86; fp32 74 us with four loads, 112 with shifted words).
+// row's memory.  (8000 x 8100 bf16, 128 x 128 blocks: 48 us, 57 with a load a
+// value; fp32 58 us, 80 with shifted words; with one load 36 and 50.)
+// WHOLE: the row does not end in the block.  Checks and addresses were a third
+// of these kernels' instructions (8000 x 8100 from 61 and 65 us), so blocks are
+// told apart once and not every chunk.
 template <class T, bool VEC> struct Chunk {
   static constexpr int kN = 16 / sizeof(T);
   union {
@@ -92,19 +119,24 @@ template <class T, bool VEC> struct Chunk {
     T raw[kN];
   };
   __device__ __forceinline__ Chunk() : words(make_uint4(0, 0, 0, 0)) {}
-  __device__ __forceinline__ void load(const T *row, int k, int cols) {
-    if (k + kN > cols || (!VEC && sizeof(T) == 4)) { // the row's end
+  // First the word that holds the first value, of all of a thread's chunks ...
+  template <bool WHOLE> __device__ __forceinline__ void fetch(const T *row, int k, int cols) {
+    if ((!WHOLE && k + kN > cols) || (!VEC && sizeof(T) == 4)) { // the row's end
 #pragma unroll
       for (int i = 0; i < kN; ++i)
-        if (k + i < cols) raw[i] = row[k + i];
-    } else if constexpr (VEC) {
-      words = __ldg(reinterpret_cast<const uint4 *>(row + k));
+        if (WHOLE || k + i < cols) raw[i] = row[k + i];
     } else {
+      words = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<uintptr_t>(row + k) & ~uintptr_t(15)));
+    }
+  }
+  // ... then the next one, which is mostly another lane's first.
+  template <bool WHOLE> __device__ __forceinline__ void align(const T *row, int k, int cols) {
+    if constexpr (!VEC && sizeof(T) == 2) {
       const uintptr_t p = reinterpret_cast<uintptr_t>(row + k);
       const uint32_t skip = p % 16;
-      const uint4 *from = reinterpret_cast<const uint4 *>(p - skip);
-      const uint4 lo = __ldg(from), hi = __ldg(from + (skip ? 1 : 0));
-      uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      if ((!WHOLE && k + kN > cols) || skip == 0) return;
+      const uint4 hi = __ldg(reinterpret_cast<const uint4 *>(p - skip + 16));
+      uint32_t w[8] = {word[0], word[1], word[2], word[3], hi.x, hi.y, hi.z, hi.w};
       if (skip & 8) {
 #pragma unroll
         for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
@@ -114,7 +146,7 @@ template <class T, bool VEC> struct Chunk {
         for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) word[i] = sizeof(T) == 4 ? w[i] : __funnelshift_r(w[i], w[i + 1], 8 * (skip & 3));
+      for (int i = 0; i < 4; ++i) word[i] = __funnelshift_r(w[i], w[i + 1], 8 * (skip & 3));
     }
   }
   // The largest |value|, as bits of its type (their order is the values', a
@@ -125,14 +157,14 @@ template <class T, bool VEC> struct Chunk {
       m = sizeof(T) == 4 ? max(m, word[i] & 0x7FFFFFFFu) : __vmaxu2(m, word[i] & 0x7FFF7FFFu);
     return m;
   }
-  __device__ __forceinline__ void store(uint8_t *row, int k, int cols, const BlockScale &s) const {
+  template <bool WHOLE> __device__ __forceinline__ void store(uint8_t *row, int k, int cols, const BlockScale &s) const {
     uint32_t u[kN / 4];
 #pragma unroll
     for (int j = 0; j < kN / 4; ++j) {
       const float v[4] = {to_f32<T>(raw[4 * j]), to_f32<T>(raw[4 * j + 1]), to_f32<T>(raw[4 * j + 2]), to_f32<T>(raw[4 * j + 3])};
       u[j] = s.quantize4(v);
     }
-    if (k + kN <= cols) { // the rows start on 16-byte boundaries
+    if (WHOLE || k + kN <= cols) { // the rows start on 16-byte boundaries
       if constexpr (kN == 8)
         *reinterpret_cast<uint2 *>(row + k) = make_uint2(u[0], u[1]);
       else
@@ -158,23 +190,33 @@ template <class T> __device__ __forceinline__ uint32_t amax_join(uint32_t a, uin
   return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b);
 }
 
-// 1 x 128 blocks: kLanes lanes a block, so that a block's scale and addresses
-// cost a quarter of a warp's instructions (with a warp a block they were most
-// of them: 8192 x 8192 bf16 103 us, 45 now; 2048 x 6400 fp32 17 us, 12.7 now,
-// 5.2 TB/s).
-constexpr int kLanes = 8;
+// 1 x 128 blocks: few lanes a block, so that a block's scale and addresses cost
+// a fraction of a warp's instructions.  (8192 x 8192 bf16: a warp a block 103
+// us, eight lanes 38, four 33, 6.2 TB/s; 2048 x 6400 fp32 10.6 us, 6.2 TB/s.)
+template <class T> constexpr int kRowLanes = sizeof(T) == 4 ? 8 : 4;
 
 template <class T, bool VEC> __global__ void __launch_bounds__(256) k_quant_rows(QuantArgs a, int kb, int blocks) {
   using C = Chunk<T, VEC>;
-  constexpr int kChunks = kScaleBlock / (kLanes * C::kN);
+  constexpr int kLanes = kRowLanes<T>, kChunks = kScaleBlock / (kLanes * C::kN);
   const long b = (long(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
   const int lane = threadIdx.x % kLanes, r = b < blocks ? int(b) / kb : 0, c = int(b) - r * kb;
   const int cols = b < blocks ? int(a.cols) : 0, k = c * kScaleBlock + lane * C::kN; // nothing past the last block
   const T *row = static_cast<const T *>(a.x) + (a.xidx ? a.xidx[r] : r) * a.ldx;
   C v[kChunks];
   uint32_t m = 0;
+  const bool whole = (c + 1) * kScaleBlock <= cols;
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) v[i].load(row, k + i * kLanes * C::kN, cols);
+    for (int i = 0; i < kChunks; ++i) v[i].template fetch<true>(row, k + i * kLanes * C::kN, cols);
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) v[i].template align<true>(row, k + i * kLanes * C::kN, cols);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+      v[i].template fetch<false>(row, k + i * kLanes * C::kN, cols);
+      v[i].template align<false>(row, k + i * kLanes * C::kN, cols);
+    }
+  }
 #pragma unroll
   for (int i = 0; i < kChunks; ++i) m = v[i].amax(m);
 #pragma unroll
@@ -183,39 +225,58 @@ template <class T, bool VEC> __global__ void __launch_bounds__(256) k_quant_rows
   const BlockScale s(amax_f32_bits<T>(m));
   if (lane == 0) a.scale[b] = s.scale;
   uint8_t *q = a.q + r * a.ldq;
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) v[i].store(q, k + i * kLanes * C::kN, cols, s);
+    for (int i = 0; i < kChunks; ++i) v[i].template store<true>(q, k + i * kLanes * C::kN, cols, s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) v[i].template store<false>(q, k + i * kLanes * C::kN, cols, s);
+  }
 }
 
 // 128 x 128 blocks: one CTA a block, its values in registers between the
-// maximum and the conversion.
-template <class T, bool VEC> __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 2 : 3) k_quant_tiles(QuantArgs a, int kb) {
+// maximum and the conversion.  Three or four CTAs an SM cover one another's
+// loads and meeting (fp32, 8000 x 8100 and one load a chunk: 50 us, 6.5 TB/s).
+// One CTA going from block to block with the next one's loads in flight had
+// half the warps and was slower (51 and 71 us where this took 45 and 66).
+template <class T, bool VEC, bool WHOLE> __device__ __forceinline__ void quant_tile(const QuantArgs &a, int rb, int c, int kb) {
   using C = Chunk<T, VEC>;
-  constexpr int kWarps = 16, kRowLanes = kScaleBlock / C::kN, kRowsAtOnce = 512 / kRowLanes;
+  constexpr int kWarps = 16, kAcross = kScaleBlock / C::kN, kRowsAtOnce = 512 / kAcross;
   constexpr int kChunks = kScaleBlock / kRowsAtOnce;
   __shared__ uint32_t part[kWarps];
-  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int rb = blockIdx.x / kb, c = blockIdx.x % kb, k = c * kScaleBlock + threadIdx.x % kRowLanes * C::kN;
-  const long r0 = long(rb) * kScaleBlock + threadIdx.x / kRowLanes;
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, cols = int(a.cols);
+  const int k = c * kScaleBlock + threadIdx.x % kAcross * C::kN;
+  const long r0 = long(rb) * kScaleBlock + threadIdx.x / kAcross;
+  const T *row = static_cast<const T *>(a.x) + r0 * a.ldx;
+  const long step = a.ldx * kRowsAtOnce;
+  const int rows = WHOLE ? kScaleBlock : int(a.rows - r0); // left from here
   C v[kChunks];
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const long r = r0 + i * kRowsAtOnce;
-    if (r < a.rows) v[i].load(static_cast<const T *>(a.x) + (a.xidx ? long(a.xidx[r]) : r) * a.ldx, k, int(a.cols));
-  }
+  for (int i = 0; i < kChunks; ++i)
+    if (WHOLE || i * kRowsAtOnce < rows) v[i].template fetch<WHOLE>(row + i * step, k, cols);
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) m = v[i].amax(m);
+  for (int i = 0; i < kChunks; ++i) {
+    if (WHOLE || i * kRowsAtOnce < rows) v[i].template align<WHOLE>(row + i * step, k, cols);
+    m = v[i].amax(m);
+  }
   m = __reduce_max_sync(0xFFFFFFFFu, amax_f32_bits<T>(m));
   if (lane == 0) part[warp] = m;
   __syncthreads();
   const BlockScale s(__reduce_max_sync(0xFFFFFFFFu, part[lane % kWarps]));
   if (threadIdx.x == 0) a.scale[long(rb) * kb + c] = s.scale;
+  uint8_t *q = a.q + r0 * a.ldq;
+  const long q_step = a.ldq * kRowsAtOnce;
 #pragma unroll
-  for (int i = 0; i < kChunks; ++i) {
-    const long r = r0 + i * kRowsAtOnce;
-    if (r < a.rows) v[i].store(a.q + r * a.ldq, k, int(a.cols), s);
-  }
+  for (int i = 0; i < kChunks; ++i)
+    if (WHOLE || i * kRowsAtOnce < rows) v[i].template store<WHOLE>(q + i * q_step, k, cols, s);
+}
+template <class T, bool VEC> __global__ void __launch_bounds__(512, sizeof(T) == 4 ? 2 : VEC ? 4 : 3) k_quant_tiles(QuantArgs a, int kb) {
+  const int rb = blockIdx.x / kb, c = blockIdx.x - rb * kb;
+  if (long(rb + 1) * kScaleBlock <= a.rows && (c + 1) * kScaleBlock <= a.cols)
+    quant_tile<T, VEC, true>(a, rb, c, kb);
+  else
+    quant_tile<T, VEC, false>(a, rb, c, kb);
 }
 
 template <class T> void launch_typed(const QuantArgs &a, cudaStream_t s) {
@@ -223,7 +284,7 @@ template <class T> void launch_typed(const QuantArgs &a, cudaStream_t s) {
   const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.ldx * sizeof(T) % 16 == 0;
   if (a.block == 1) {
     const int blocks = int(a.rows * kb); // the callers keep it in 31 bits
-    const unsigned grid = (unsigned(blocks) + 256 / kLanes - 1) / (256 / kLanes);
+    const unsigned grid = (unsigned(blocks) + 256 / kRowLanes<T> - 1) / (256 / kRowLanes<T>);
     if (vec)
       k_quant_rows<T, true><<<grid, 256, 0, s>>>(a, kb, blocks);
     else
