@@ -20,13 +20,14 @@
 // one a lane; values above the last that matters gather in shared memory and
 // are sorted and merged in 32 at a time, so that most values cost a comparison.
 // (Taking the best out one by one with warp-wide maxima cost 120 instructions
-// a beam and row: 64 x 32 x 264 38 us, 15.8 now.)
+// a beam and row: 64 x 32 x 264 38 us, 15.9 now.)
 #include "beam_kernels.h"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <stdexcept>
 
 namespace ngb {
@@ -59,12 +60,11 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// exp of N values <= 0, each to about 1e-12 of it: 2^n times the Taylor
+// exp of N values in [-140, 0], each to about 1e-12 of it: 2^n times the Taylor
 // polynomial of degree 10 on |r| <= ln 2 / 2 (its remainder is below 3e-13).
-// Below -80, and for a NaN, it is 0: against a sum of at least 1 such a term
-// has no bit.  The values go through each step together, which the volatile
-// statements keep (9 values of a warp: 916 clocks; one after the other, as the
-// compiler orders plain code, 1,492).
+// The values go through each step together, which the volatile statements keep
+// (9 values of a warp: 916 clocks; one after the other, as the compiler orders
+// plain code, 1,492).
 __constant__ double kTaylor[11] = {1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720, 1.0 / 120,
                                    1.0 / 24,      1.0 / 6,      0.5,         1.0,        1.0};
 __constant__ double kExp[3] = {6755399441055744.0, // 1.5 * 2^52: the sum's low word is the nearest integer
@@ -76,12 +76,8 @@ __device__ __forceinline__ double step_fma(double a, double b, double c) {
 }
 template <int N> __device__ __forceinline__ void exp_below(double (&v)[N]) {
   double t[N], p[N];
-  bool counts[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    counts[i] = v[i] >= -80.0;
-    t[i] = step_fma(v[i], kExp[1], kExp[0]);
-  }
+  for (int i = 0; i < N; ++i) t[i] = step_fma(v[i], kExp[1], kExp[0]);
 #pragma unroll
   for (int i = 0; i < N; ++i) v[i] = step_fma(-__dsub_rn(t[i], kExp[0]), kExp[2], v[i]);
 #pragma unroll
@@ -92,24 +88,29 @@ template <int N> __device__ __forceinline__ void exp_below(double (&v)[N]) {
     for (int i = 0; i < N; ++i) p[i] = step_fma(p[i], v[i], kTaylor[k]);
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    v[i] = counts[i] ? __hiloint2double(__double2hiint(p[i]) + (__double2loint(t[i]) << 20), __double2loint(p[i])) : 0.0;
+    v[i] = __hiloint2double(__double2hiint(p[i]) + (__double2loint(t[i]) << 20), __double2loint(p[i]));
 }
 
 // Sums of exponentials against the largest logit seen, as its key (0: none).
+// Terms 80 or more below it are left out: against a sum of at least 1 they have
+// no bit.  With a top of kBadKey or more the sum means nothing.
 struct LogSum {
   uint32_t top = 0;
   double sum = 0;
   __device__ __forceinline__ void raise(uint32_t to) { // to >= top
     if (to == top) return;
     double d[1] = {__dsub_rn(double(logit_of(top)), double(logit_of(to)))};
+    const bool counts = top && d[0] >= -80.0;
     exp_below(d);
-    sum = top ? __dmul_rn(sum, d[0]) : 0.0;
+    sum = counts ? __dmul_rn(sum, d[0]) : 0.0;
     top = to;
   }
   // Adds N logits' terms; none above top, -inf for none.  TOGETHER at a time.
+  // The bound is one fp32 subtraction: rounded, it still lies within 140 of top.
   template <int TOGETHER, int N> __device__ __forceinline__ void add(const float (&x)[N]) {
     static_assert(N % TOGETHER == 0, "values");
-    const double m = logit_of(top);
+    const float most = logit_of(top), least = top ? __fsub_rn(most, 80.f) : INFINITY;
+    const double m = most;
 #pragma unroll
     for (int i = 0; i < N; i += TOGETHER) {
       double d[TOGETHER];
@@ -117,7 +118,8 @@ struct LogSum {
       for (int j = 0; j < TOGETHER; ++j) d[j] = __dsub_rn(double(x[i + j]), m);
       exp_below(d);
 #pragma unroll
-      for (int j = 0; j < TOGETHER; ++j) sum = __dadd_rn(sum, d[j]);
+      for (int j = 0; j < TOGETHER; ++j)
+        if (x[i + j] >= least) sum = __dadd_rn(sum, d[j]);
     }
   }
   __device__ __forceinline__ void join_warp() {
@@ -148,8 +150,19 @@ __device__ __forceinline__ uint64_t sort32(uint64_t v) {
     for (int j = k / 2; j > 0; j /= 2) v = exchange(v, j, ((lane & j) == 0) == ((lane & k) == 0));
   return v;
 }
-// The same of plain keys.
-__device__ __forceinline__ uint32_t sort32_keys(uint32_t v) {
+// A key that at least n of the lanes' keys reach, the n-th if they differ: the
+// largest removed n - 1 times, or for more from the sorted keys.  (4 beams of
+// 264: 4.3 us, always sorting 4.5; one removal is two instructions.)
+constexpr int kRemove = 16;
+__device__ __forceinline__ uint32_t nth_key(uint32_t v, int n) {
+  if (n <= kRemove) {
+    uint32_t most = __reduce_max_sync(kAll, v);
+    for (int i = 1; i < n; ++i) {
+      v = v == most ? 0 : v;
+      most = __reduce_max_sync(kAll, v);
+    }
+    return most;
+  }
   const int lane = threadIdx.x % 32;
 #pragma unroll
   for (int k = 2; k <= 32; k *= 2)
@@ -158,7 +171,7 @@ __device__ __forceinline__ uint32_t sort32_keys(uint32_t v) {
       const uint32_t o = __shfl_xor_sync(kAll, v, j);
       v = ((lane & j) == 0) == ((lane & k) == 0) ? max(v, o) : min(v, o);
     }
-  return v;
+  return __shfl_sync(kAll, v, n - 1);
 }
 // The best 32 of two sorted lists, sorted.
 __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b) {
@@ -198,49 +211,75 @@ struct Best {
   }
 };
 
+// The larger of two, a NaN if either is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Streams over tokens [v0, v1) of a row.  kStep values a lane are in flight;
-// nine cover the byte vocabulary (264) in one step.
-constexpr int kStep = 9;
-template <class T, int TOGETHER>
+// nine cover the byte vocabulary (264) in one step.  A value costs its
+// exponential, a maximum and a comparison; keys are made of the few that pass,
+// and only a row's last step checks its end.
+constexpr int kStep = 9, kStepValues = 32 * kStep;
+template <bool WHOLE, class T>
+__device__ __forceinline__ void load_step(T (&to)[kStep], const T *x, int v, int v1) {
+  const int at = v + threadIdx.x % 32;
+#pragma unroll
+  for (int i = 0; i < kStep; ++i) to[i] = x[WHOLE ? at + 32 * i : min(at + 32 * i, v1 - 1)];
+}
+template <class T> __device__ __forceinline__ void load_step(T (&to)[kStep], const T *x, int v, int v1) {
+  if (v1 - v >= kStepValues)
+    load_step<true>(to, x, v, v1);
+  else // past the end: the last value, which is not used
+    load_step<false>(to, x, v, v1);
+}
+template <class T, int TOGETHER, bool SHARED>
 __device__ __forceinline__ void stream_row(const BeamArgs &a, const T *x, int v0, int v1, LogSum &ls, Best &best,
-                                           uint64_t *wait) {
+                                           uint64_t *wait, uint32_t *shared_bar) {
   const int lane = threadIdx.x % 32;
   T next[kStep];
-  const auto load = [&](int v) { // past the end: the last value, which is not used
+  if (v0 < v1) load_step(next, x, v0, v1);
+  for (int v = v0; v < v1; v += kStepValues) {
+    float logit[kStep], top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) next[i] = x[min(v + 32 * i + lane, v1 - 1)];
-  };
-  if (v0 < v1) load(v0);
-  for (int v = v0; v < v1; v += 32 * kStep) {
-    float logit[kStep];
-    uint32_t key[kStep], top = 0;
+    for (int i = 0; i < kStep; ++i) logit[i] = to_f32<T>(next[i]);
     if (a.allowed) {
       uint8_t ok[kStep];
+      load_step(ok, a.allowed, v, v1);
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) ok[i] = a.allowed[min(v + 32 * i + lane, v1 - 1)];
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) logit[i] = ok[i] && v + 32 * i + lane < v1 ? to_f32<T>(next[i]) : -INFINITY;
-    } else {
-#pragma unroll
-      for (int i = 0; i < kStep; ++i) logit[i] = v + 32 * i + lane < v1 ? to_f32<T>(next[i]) : -INFINITY;
+      for (int i = 0; i < kStep; ++i) logit[i] = ok[i] ? logit[i] : -INFINITY;
     }
-    if (v + 32 * kStep < v1) load(v + 32 * kStep);
+    if (v1 - v < kStepValues) {
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) key[i] = key_of(logit[i]), top = max(top, key[i]);
-    if (top > ls.top) ls.raise(top);
+      for (int i = 0; i < kStep; ++i) logit[i] = v + 32 * i + lane < v1 ? logit[i] : -INFINITY;
+    }
+    if (v + kStepValues < v1) load_step(next, x, v + kStepValues, v1);
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) top = max_nan(top, logit[i]);
+    const uint32_t top_key = key_of(top);
+    if (top_key > ls.top) ls.raise(top_key);
     ls.add<TOGETHER>(logit);
     if (v == v0) // of the lanes' largest, the beams-th: at least `beams` values reach it
-      best.bar = uint64_t(__shfl_sync(kAll, sort32_keys(top), a.beams - 1)) << 32;
+      best.bar = uint64_t(nth_key(top_key, a.beams)) << 32;
+    if constexpr (SHARED) { // `beams` values that another warp of the row has seen reach its bar
+      uint32_t key = entry_key(best.bar);
+      if (lane == 0) key = max(key, atomicMax(shared_bar, key));
+      const uint64_t most = uint64_t(__shfl_sync(kAll, key, 0)) << 32;
+      best.bar = best.bar > most ? best.bar : most;
+    }
     // A lane's values that may matter, one a round: few do.
+    const float bar = fmaxf(logit_of(entry_key(best.bar)), -FLT_MAX);
     uint32_t some = 0;
 #pragma unroll
-    for (int i = 0; i < kStep; ++i) some |= uint32_t(key[i] && key[i] >= entry_key(best.bar)) << i;
+    for (int i = 0; i < kStep; ++i) some |= uint32_t(logit[i] >= bar) << i;
     while (__any_sync(kAll, some != 0)) {
       const int which = __ffs(some) - 1;
-      uint32_t k = 0;
+      float l = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kStep; ++i) k = i == which ? key[i] : k;
-      best.push(entry(k, v + 32 * which + lane), wait, a.beams);
+      for (int i = 0; i < kStep; ++i) l = i == which ? logit[i] : l;
+      best.push(entry(key_of(l), v + 32 * which + lane), wait, a.beams);
       some &= some - 1;
     }
   }
@@ -377,8 +416,8 @@ template <class T, int THREADS> __global__ void __launch_bounds__(THREADS) k_bea
   LogSum ls;
   Best best;
   if (beam.exists && !beam.finished) {
-    stream_row<T, THREADS == 512 ? 9 : 3>(a, static_cast<const T *>(a.logits) + row * a.ld, 0, a.vocab, ls, best,
-                                          shares[w].wait);
+    stream_row<T, THREADS == 512 ? 9 : 3, false>(a, static_cast<const T *>(a.logits) + row * a.ld, 0, a.vocab, ls, best,
+                                                 shares[w].wait, nullptr);
     ls.join_warp();
   }
   finish_group(a, blockIdx.x, beam, ls, best.mine, shares);
@@ -402,7 +441,6 @@ struct Slice {
 __host__ __device__ inline bool in_slices(long rows, int vocab) {
   return rows < 8 * 148 && vocab > (rows < 256 ? 1024 : 2048);
 }
-constexpr int kStepValues = 32 * kStep;
 __host__ __device__ inline int row_steps(int vocab) { return (vocab + kStepValues - 1) / kStepValues; }
 // Slices of a row: so many steps a warp that all CTAs run at once (three an
 // SM), and no more slices than these steps fill.
@@ -415,7 +453,9 @@ __host__ __device__ inline int slice_count(long rows, int vocab) {
 template <class T> __global__ void __launch_bounds__(32 * kSliceWarps, 3) k_beam_slice(BeamArgs a, int slices) {
   __shared__ uint64_t wait[kSliceWarps][kWaiting];
   __shared__ double sums[kSliceWarps];
-  __shared__ uint32_t tops[kSliceWarps];
+  __shared__ uint32_t tops[kSliceWarps], bar;
+  if (threadIdx.x == 0) bar = 0;
+  __syncthreads();
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const long row = blockIdx.x / slices;
   const int slice = blockIdx.x % slices;
@@ -425,8 +465,8 @@ template <class T> __global__ void __launch_bounds__(32 * kSliceWarps, 3) k_beam
   const long part = slice * kSliceWarps + warp, parts = slices * kSliceWarps, steps = row_steps(a.vocab);
   LogSum ls;
   Best best;
-  stream_row<T, 9>(a, static_cast<const T *>(a.logits) + row * a.ld, int(min(long(a.vocab), part * steps / parts * kStepValues)),
-                   int(min(long(a.vocab), (part + 1) * steps / parts * kStepValues)), ls, best, wait[warp]);
+  stream_row<T, 9, true>(a, static_cast<const T *>(a.logits) + row * a.ld, int(min(long(a.vocab), part * steps / parts * kStepValues)),
+                   int(min(long(a.vocab), (part + 1) * steps / parts * kStepValues)), ls, best, wait[warp], &bar);
   ls.join_warp();
   if (lane == 0) sums[warp] = ls.sum, tops[warp] = ls.top;
   for (int step = 1; step < kSliceWarps; step *= 2) { // the warps' lists, in pairs

@@ -143,6 +143,29 @@ def test_select_ties_go_to_the_lower_index(vocab):
         check_select(row.expand(2 * beams, vocab).contiguous().bfloat16(), scores)
 
 
+@pytest.mark.parametrize('vocab', [100, 264, 4000])
+@pytest.mark.parametrize('centre', [-2.0 ** 31, -2.0 ** 30, 2.0 ** 24, 2.0 ** 29, 2.0 ** 30 + 64, 2.0 ** 31, 1e30, -1e30])
+def test_select_far_from_zero(centre, vocab):
+    """Logits whose fp32 steps are of the size of the terms that still count, or larger.
+
+    lse = m + log(sum) is one 64-bit rounding at |m| <= 2^31 + 2^12, and two sums that differ in
+    their last bits may round to neighbours, 2^-21 apart; the score's fp32 rounding is 2^-24 of it.
+    At 1e30 log(sum) < 9 vanishes on both sides.  Scores 1 apart keep the beams' order clear of it."""
+    rng = np.random.default_rng(vocab)
+    step = np.spacing(np.float32(abs(centre)))
+    beams = 5
+    logits = np.float32(centre) + step * rng.integers(-6, 1, (2 * beams, vocab)).astype(np.float32)
+    assert logits.dtype == np.float32
+    scores = -np.arange(2 * beams, dtype=np.float32).reshape(2, beams) * 1.25
+    allowed = rng.random(vocab) < 0.9
+    got = decoding.beam_select(torch.from_numpy(logits).cuda(), torch.from_numpy(scores).cuda(), None,
+                               torch.from_numpy(allowed).cuda(), None, 0)
+    want = select_64(logits, scores, None, allowed, None, 0)
+    np.testing.assert_allclose(got[0].cpu().numpy(), want[0], rtol=2.0 ** -23, atol=2.0 ** -20)
+    for have, need in zip(got[1:], want[1:]):
+        assert np.array_equal(have.cpu().numpy(), need)
+
+
 @pytest.mark.parametrize('vocab', [70, 264, 5000])
 def test_select_masks_and_bad_values(vocab):
     rng, logits, scores = inputs(vocab, 6, 5, vocab)
