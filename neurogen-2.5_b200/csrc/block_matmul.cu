@@ -155,12 +155,19 @@ __global__ void __launch_bounds__(32 * kVecWarps, CTAS) k_block_vec(BlockMatmulA
 // More rows: the tensor cores proper.  A tile is 128 rows of a (TMEM lanes) x
 // TN weight rows (TMEM columns).  One thread streams the blocks of 128 bytes
 // along k by TMA (SWIZZLE_128B, one swizzle atom a row), one issues each
-// block's four MMAs (M=128, N=TN, K=32) into a TMEM accumulator of its own, two warps stage the rows' scales, and 4 or 8 warps add the
-// finished accumulators, scaled, to the sums in their registers.  TN divides
-// 128 or is 256 in two halves, so a warp's columns share one weight scale and
-// a thread's row one scale of a: a block's addition is one packed fma a pair
-// of columns and nothing else.  The next 32 columns are on their way from
-// TMEM while the last ones are added.
+// block's four MMAs (M=128, N=TN, K=32) into a TMEM accumulator of its own,
+// two warps stage the rows' scales, and 4 or 8 warps add the finished
+// accumulators, scaled, to the sums in their registers.  TN divides 128 or is
+// 256 in two halves, so a warp's columns share one weight scale and a thread's
+// row one scale of a: a block's addition is one packed fma a pair of columns
+// and nothing else.  A warp reads 64 columns at a time and gives a set back
+// before it adds the last of them.
+//
+// What bounds large products is the accumulators' way out: while MMAs run, one
+// of 128 x 256 takes some 700 clocks to read, and its own MMAs 541 (8192 x 8192
+// x 4096: 255 us, tensor pipe 56%).  Pairs of CTAs on one tile (cta_group::2)
+// halve the weights' copies and not that, and hand back over the cluster, 500
+// clocks later: 512 us.
 //
 // The roles meet (mbarriers) once for kPair blocks: a meeting costs the MMAs'
 // thread some 400 clocks, more than a block's MMAs take when TN is small
@@ -241,15 +248,14 @@ __device__ __forceinline__ void tmem_issue32(uint32_t addr, uint32_t (&r)[32]) {
                  "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
                : "r"(addr));
 }
-__device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]),
-                 "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]),
-                 "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
-                 "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]),
-                 "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29])
-               ::"memory");
-  asm volatile("" : "+r"(r[30]), "+r"(r[31]));
+__device__ __forceinline__ void hold(uint32_t *r) {
+  asm volatile(""
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]));
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&r)[2][32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  hold(r[0]), hold(r[0] + 16), hold(r[1]), hold(r[1] + 16);
 }
 __device__ __forceinline__ uint64_t pair(float v) {
   uint64_t p;
@@ -490,11 +496,16 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
     int left = first < tiles ? ((tiles - 1 - first) / stride + 1) * sets : 0; // still to add
     int acc = 0, chunk = 0; // set in turn, scale buffers taken so far
     uint32_t parity = 0;    // of the ring's round
+    // 32 columns i of a set: of its block i / kPer.
+    constexpr int kPer = S::kCols / 32;
+    const auto load = [&](int i) {
+      tmem_issue32(from + acc * (S::kPair * TN) + i / kPer * TN + i % kPer * 32, d[i % 2]);
+    };
     // The first columns of the set in turn, once it is ready, on their way to registers.
     const auto begin = [&] {
       alive = wait_warp(ready + 8 * acc, parity, abort_s);
       fence_after();
-      if (alive) tmem_issue32(from + acc * (S::kPair * TN), d[0]);
+      if (alive) load(0), load(1);
     };
     if (alive && left) begin();
     for (int tile = first; tile < tiles && alive; tile += stride) {
@@ -505,33 +516,34 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
         alive = wait_warp(sfull + 8 * buf, (chunk / 2) & 1, abort_s);
         const float *sa = scales_a + buf * kScaleChunk * kTileM + row, *sw = scales_w + buf * kScaleChunk * S::kGroups + group;
         for (int b = min(kScaleChunk, kb1 - c); b > 0 && alive; b -= S::kPair) {
-          const uint32_t at = from + acc * (S::kPair * TN);
+          const int blocks = min(b, S::kPair);
+          uint64_t scale[S::kPair];
 #pragma unroll
-          for (int u = 0; u < S::kPair; ++u, sa += kTileM, sw += S::kGroups) {
-            if (u >= b) continue;
-            const uint64_t scale = pair(__fmul_rn(*sa, *sw));
+          for (int u = 0; u < S::kPair; ++u, sa += kTileM, sw += S::kGroups)
+            scale[u] = u < blocks ? pair(__fmul_rn(*sa, *sw)) : 0;
 #pragma unroll
-            for (int j = 0; j < S::kCols; j += 32) {
-              const int q = (u * S::kCols + j) / 32 % 2;
-              // Set taken: all of it is in registers; the next begins in d[0], which must be free.
-              const auto next_set = [&] {
-                if (--left) begin();
-              };
-              tmem_wait32(d[q]);
-              const bool last = j + 32 == S::kCols && u + 1 >= min(b, S::kPair);
-              if (!last) {
-                tmem_issue32(at + u * TN + (j + 32 < S::kCols ? j + 32 : TN), d[1 - q]);
-              } else {
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(taken + 8 * acc);
-                acc = acc + 1 == S::kAccs ? 0 : acc + 1;
-                parity ^= acc == 0;
-                if (q == 1) next_set();
+          for (int i = 0; i < S::kPair * kPer; i += 2) {
+            if (i / kPer >= blocks) continue;
+            const bool last = i + 2 >= blocks * kPer; // of the set
+            tmem_wait(d);
+            if (last) {
+              fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(taken + 8 * acc);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int u = (i + h) / kPer, j = (i + h) % kPer * 32;
+              if (u < blocks) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) fma2(sum[(j + e) / 2], d[h][e], d[h][e + 1], scale[u]);
               }
-#pragma unroll
-              for (int i = 0; i < 32; i += 2) fma2(sum[(j + i) / 2], d[q][i], d[q][i + 1], scale);
-              if (last && q == 0) next_set();
+              if (!last) load(i + 2 + h);
+            }
+            if (last) {
+              acc = acc + 1 == S::kAccs ? 0 : acc + 1;
+              parity ^= acc == 0;
+              if (--left) begin();
             }
           }
         }
