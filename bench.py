@@ -657,7 +657,9 @@ def cpu_baseline_lang(name, toks, budget_s):
     import multiprocessing
     from concurrent.futures import ThreadPoolExecutor
     from neurogen_b200.language import LanguageConfig
-    from oracle.lang import RefEngine, seeded_weights
+    from oracle.lang import REF_LIB, RefEngine, seeded_weights
+    if not REF_LIB.is_file():
+        return {'unavailable': 'the reference native CPU library (oracle/_ref) is not built here'}
     cfg = LanguageConfig()
     w = seeded_weights()
     threads = 1 if name == 'bc250' else multiprocessing.cpu_count()
@@ -749,7 +751,9 @@ def reference_record(name, args, world, steps, warmup):
         metric = METRIC_TICKS
     else:
         from concurrent.futures import ThreadPoolExecutor
-        from oracle.lang import RefEngine, seeded_weights
+        from oracle.lang import REF_LIB, RefEngine, seeded_weights
+        if not REF_LIB.is_file():
+            return {'impl': 'reference', 'unavailable': 'the reference native CPU library (oracle/_ref) is not built here'}
 
         class Cfg:
             columns, width, regions, ticks, idle_steps = 32, 768, 4, 2, 1
