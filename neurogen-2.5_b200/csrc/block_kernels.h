@@ -17,6 +17,20 @@ inline long block_row_bytes(long cols) { return (cols + 15) / 16 * 16; }
 inline long scale_blocks(long n) { return (n + kScaleBlock - 1) / kScaleBlock; }
 inline size_t elem_size(Elem t) { return t == Elem::f32 ? 4 : 2; }
 
+// Block b of a matrix of `blocks` <= 2^31 - 1 blocks of 1 x 128, kb of them a row
+// of cols <= 2^30 columns.  A block past the last one has row 0 and no columns:
+// all its values lie past its end, and no index is formed from its number, which
+// may pass 31 bits.
+struct RowBlock {
+  int row, block, cols;
+  bool whole; // the row does not end in the block
+};
+__host__ __device__ inline RowBlock row_block(long b, long blocks, int kb, long cols) {
+  if (b >= blocks) return {0, 0, 0, false};
+  const int row = int(b) / kb, block = int(b) - row * kb;
+  return {row, block, int(cols), (block + 1) * kScaleBlock <= int(cols)};
+}
+
 struct QuantArgs {
   const void *x; // [rows] rows of cols, row stride ldx elements
   Elem type;

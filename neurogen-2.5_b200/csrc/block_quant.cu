@@ -199,12 +199,11 @@ template <class T, bool VEC> __global__ void __launch_bounds__(256) k_quant_rows
   using C = Chunk<T, VEC>;
   constexpr int kLanes = kRowLanes<T>, kChunks = kScaleBlock / (kLanes * C::kN);
   const long b = (long(blockIdx.x) * blockDim.x + threadIdx.x) / kLanes;
-  const int lane = threadIdx.x % kLanes, r = b < blocks ? int(b) / kb : 0, c = int(b) - r * kb;
-  const int cols = b < blocks ? int(a.cols) : 0, k = c * kScaleBlock + lane * C::kN; // nothing past the last block
+  const auto [r, c, cols, whole] = row_block(b, blocks, kb, a.cols);
+  const int lane = threadIdx.x % kLanes, k = c * kScaleBlock + lane * C::kN;
   const T *row = static_cast<const T *>(a.x) + (a.xidx ? a.xidx[r] : r) * a.ldx;
   C v[kChunks];
   uint32_t m = 0;
-  const bool whole = (c + 1) * kScaleBlock <= cols;
   if (whole) {
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) v[i].template fetch<true>(row, k + i * kLanes * C::kN, cols);
