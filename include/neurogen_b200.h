@@ -333,8 +333,9 @@ int ng_block_quantize(int device, const void *x, int dtype, int64_t rows, int64_
 /* y[m][n] = sum_k a[m][k] w[n][k] (+ bias[n]) (+ add_scale * add[m][n]), a with
  * a scale for each 1 x 128 block, w for each 128 x 128 block.  fp32 sums: the
  * bytes' products of one block of 128 on the tensor cores, then the blocks in
- * a fixed order; rounded once to y's type.  The result is a function of the
- * operands and sizes alone.  bias and add are fp32 and may be NULL; y may be
+ * a fixed order; rounded once to y's type.  Any finite scales: a block counts
+ * a_scale * w_scale * its sum although the scales' product alone may leave
+ * fp32's range.  The result is a function of the operands and sizes alone.  bias and add are fp32 and may be NULL; y may be
  * add when it is fp32 with the same stride. */
 int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale, const void *w, int64_t ldw,
                     const float *w_scale, int64_t m, int64_t n, int64_t k, const float *bias, const float *add,

@@ -14,6 +14,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <climits>
 #include <cmath>
 #include <cstdlib>
@@ -38,6 +39,33 @@ __device__ __forceinline__ void finish(const BlockMatmulArgs &a, int m, int n, f
   if (a.bias) v = __fadd_rn(v, a.bias[n]);
   if (a.add) v = __fmaf_rn(a.add_scale, a.add[long(m) * a.ldadd + n], v);
   store_elem(a.y, a.type, long(m) * a.ldy + n, v);
+}
+
+// A block's sum d counts sa sw d.  d is 0 or lies between 2^-18 and 2^25, so
+// that can be an ordinary number where s = sa sw overflows or is subnormal
+// (bytes that use little of their range, values near fp32's ends).  There d
+// first takes a power of two p = 2^100 or 2^-100, exactly, and s = sa sw / p
+// rounds as a normal number: where even that leaves the range, the result is
+// an infinity (or 0, for d = 0) or rounds to nothing.
+struct ScalePair {
+  float s, p;
+};
+__device__ __forceinline__ bool is_normal(float v) { // neither 0 nor subnormal nor infinite nor NaN
+  return 2 * __float_as_uint(v) - (1u << 24) < (254u << 24);
+}
+__device__ __forceinline__ ScalePair scale_pair(float sa, float sw) {
+  const float s = __fmul_rn(sa, sw);
+  const auto counts = [](float v) { return v != 0.f && fabsf(v) <= FLT_MAX; };
+  if (is_normal(s) || !counts(sa) || !counts(sw)) return {s, 1.f};
+  const bool large = fabsf(s) > 1.f;
+  const float half = large ? 0x1p-50f : 0x1p50f; // exact on both: neither is far on the other side
+  const float rest = __fmul_rn(__fmul_rn(sa, half), __fmul_rn(sw, half));
+  return {fminf(fmaxf(rest, -FLT_MAX), FLT_MAX), large ? 0x1p100f : 0x1p-100f};
+}
+
+// Outside 2^-63 .. 2^63: two scales within have a normal product.
+__device__ __forceinline__ bool is_far(float v) {
+  return (__float_as_uint(v) & 0x7FFFFFFFu) - (64u << 23) > (126u << 23);
 }
 
 // Sixteen consecutive bytes of a row from column k, zero past the row's end.
@@ -115,25 +143,45 @@ __global__ void __launch_bounds__(32 * kVecWarps, CTAS) k_block_vec(BlockMatmulA
 #pragma unroll
       for (int i = 0; i < NT; ++i) v[u].sa[i][0] = sa[i][0][b], v[u].sa[i][1] = sa[i][1][b];
     }
+    bool odd = false; // some scale product here needs two factors (ScalePair)
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (b0 + u * kVecWarps >= kb) continue;
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint4 x = v[u].w[0][h], y = v[u].w[1][h], z = v[u].a[i][h];
-          mma_e4m3(d, x.x, y.x, x.y, y.y, z.x, z.y);
-          mma_e4m3(d, x.z, y.z, x.w, y.w, z.z, z.w);
-        }
-        const float s0 = __fmul_rn(v[u].sw, v[u].sa[i][0]), s1 = __fmul_rn(v[u].sw, v[u].sa[i][1]);
-        sum[i][0] = __fmaf_rn(s0, d[0], sum[i][0]);
-        sum[i][1] = __fmaf_rn(s1, d[1], sum[i][1]);
-        sum[i][2] = __fmaf_rn(s0, d[2], sum[i][2]);
-        sum[i][3] = __fmaf_rn(s1, d[3], sum[i][3]);
-      }
+        for (int j = 0; j < 2; ++j) odd |= !is_normal(__fmul_rn(v[u].sa[i][j], v[u].sw));
     }
+    const auto blocks = [&](auto split) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (b0 + u * kVecWarps >= kb) continue;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint4 x = v[u].w[0][h], y = v[u].w[1][h], z = v[u].a[i][h];
+            mma_e4m3(d, x.x, y.x, x.y, y.y, z.x, z.y);
+            mma_e4m3(d, x.z, y.z, x.w, y.w, z.z, z.w);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float s = __fmul_rn(v[u].sa[i][j], v[u].sw);
+            if constexpr (split.value) {
+              const ScalePair f = scale_pair(v[u].sa[i][j], v[u].sw);
+              s = f.s, d[j] = __fmul_rn(f.p, d[j]), d[j + 2] = __fmul_rn(f.p, d[j + 2]);
+            }
+            sum[i][j] = __fmaf_rn(s, d[j], sum[i][j]);
+            sum[i][j + 2] = __fmaf_rn(s, d[j + 2], sum[i][j + 2]);
+          }
+        }
+      }
+    };
+    if (__any_sync(0xFFFFFFFFu, odd))
+      blocks(std::true_type());
+    else
+      blocks(std::false_type());
   }
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
@@ -233,6 +281,16 @@ __device__ __forceinline__ void fma2(uint64_t &sum, uint32_t d0, uint32_t d1, ui
   uint64_t d;
   asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
   asm volatile("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(d), "l"(scale));
+}
+// The same where the scale is held in two factors (ScalePair).
+__device__ __forceinline__ void fma2_split(uint64_t &sum, uint32_t d0, uint32_t d1, uint64_t scale, uint64_t power) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(d0), "r"(d1));
+  asm volatile("{\n\t.reg .b64 t;\n\t"
+               "mul.rn.f32x2 t, %1, %3;\n\t"
+               "fma.rn.f32x2 %0, t, %2, %0;\n\t}"
+               : "+l"(sum)
+               : "l"(d), "l"(scale), "l"(power));
 }
 // 32 consecutive TMEM columns of this thread's lane: the load, and the wait
 // for every load issued, which the registers pass through so that no use of
@@ -430,6 +488,8 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
   uint64_t *bars = reinterpret_cast<uint64_t *>(scales_w + 2 * kScaleChunk * S::kGroups);
   volatile uint32_t *tmem_slot = reinterpret_cast<volatile uint32_t *>(bars + S::kBars);
   volatile int *abort_s = reinterpret_cast<volatile int *>(tmem_slot + 1);
+  // [2][2], of a buffer and of the warp that filled it: a scale product may need two factors.
+  volatile uint8_t *far_scales = reinterpret_cast<volatile uint8_t *>(abort_s + 1);
   // One value for the whole warp, known as such: the roles' branches are uniform.
   const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid / 32, 0), lane = tid % 32;
   const int kb = (a.k + kScaleBlock - 1) / kScaleBlock;
@@ -444,7 +504,7 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
 
   const bool stalled = stall_test != 0; // test switch: the path of a wait that ran out, with nothing in flight
   // Scales of 16 blocks along k from b on: lane = block and one of four rows
-  // (two warps), rows and blocks out of range count nothing.
+  // (two warps); 1 for rows and blocks out of range, whose bytes are zeros.
   const int quarter = (warp - kScaleWarp) * 2 + lane / kScaleChunk, at = lane % kScaleChunk;
   constexpr int kBatch = S::kGroups == 1 ? 32 : 16; // loads in flight together
   float v[kBatch], vw;
@@ -452,8 +512,8 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
     const int b = c + at, m = tile / tiles_n * kTileM + quarter + r, n = tile % tiles_n * TN + quarter * S::kCols;
     const float *from = a.a_scale + long(m) * kb + b;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) v[i] = b < kb1 && m + 4 * i < a.m ? from[4 * i * long(kb)] : 0.f;
-    vw = quarter < S::kGroups && b < kb1 && n < a.n ? a.w_scale[long(n / kScaleBlock) * kb + b] : 0.f;
+    for (int i = 0; i < kBatch; ++i) v[i] = b < kb1 && m + 4 * i < a.m ? from[4 * i * long(kb)] : 1.f;
+    vw = quarter < S::kGroups && b < kb1 && n < a.n ? a.w_scale[long(n / kScaleBlock) * kb + b] : 1.f;
   };
   // Before the CTA meets, only what does not make it wait.
   if (warp == kCopyWarp) {
@@ -515,38 +575,59 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
         const int buf = chunk % 2;
         alive = wait_warp(sfull + 8 * buf, (chunk / 2) & 1, abort_s);
         const float *sa = scales_a + buf * kScaleChunk * kTileM + row, *sw = scales_w + buf * kScaleChunk * S::kGroups + group;
-        for (int b = min(kScaleChunk, kb1 - c); b > 0 && alive; b -= S::kPair) {
-          const int blocks = min(b, S::kPair);
-          uint64_t scale[S::kPair];
+        // far: some scale of the chunk lies outside 2^-63 .. 2^63, so a product of two may leave the
+        // normal range.  Two loops, told apart once a chunk (8192 x 8192 x 4096: 252 us, as without
+        // the second; the split form in the one loop 282).
+        const auto add_chunk = [&](auto far) {
+          for (int b = min(kScaleChunk, kb1 - c); b > 0 && alive; b -= S::kPair) {
+            const int blocks = min(b, S::kPair);
+            uint64_t scale[S::kPair];
+            uint64_t power[S::kPair];
 #pragma unroll
-          for (int u = 0; u < S::kPair; ++u, sa += kTileM, sw += S::kGroups)
-            scale[u] = u < blocks ? pair(__fmul_rn(*sa, *sw)) : 0;
-#pragma unroll
-          for (int i = 0; i < S::kPair * kPer; i += 2) {
-            if (i / kPer >= blocks) continue;
-            const bool last = i + 2 >= blocks * kPer; // of the set
-            tmem_wait(d);
-            if (last) {
-              fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(taken + 8 * acc);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int u = (i + h) / kPer, j = (i + h) % kPer * 32;
-              if (u < blocks) {
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) fma2(sum[(j + e) / 2], d[h][e], d[h][e + 1], scale[u]);
+            for (int u = 0; u < S::kPair; ++u, sa += kTileM, sw += S::kGroups) {
+              if constexpr (far.value) {
+                const ScalePair s = u < blocks ? scale_pair(*sa, *sw) : ScalePair{0.f, 1.f};
+                scale[u] = pair(s.s), power[u] = pair(s.p);
+              } else {
+                scale[u] = u < blocks ? pair(__fmul_rn(*sa, *sw)) : 0;
               }
-              if (!last) load(i + 2 + h);
             }
-            if (last) {
-              acc = acc + 1 == S::kAccs ? 0 : acc + 1;
-              parity ^= acc == 0;
-              if (--left) begin();
+#pragma unroll
+            for (int i = 0; i < S::kPair * kPer; i += 2) {
+              if (i / kPer >= blocks) continue;
+              const bool last = i + 2 >= blocks * kPer; // of the set
+              tmem_wait(d);
+              if (last) {
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(taken + 8 * acc);
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int u = (i + h) / kPer, j = (i + h) % kPer * 32;
+                if (u < blocks) {
+#pragma unroll
+                  for (int e = 0; e < 32; e += 2) {
+                    if constexpr (far.value)
+                      fma2_split(sum[(j + e) / 2], d[h][e], d[h][e + 1], scale[u], power[u]);
+                    else
+                      fma2(sum[(j + e) / 2], d[h][e], d[h][e + 1], scale[u]);
+                  }
+                }
+                if (!last) load(i + 2 + h);
+              }
+              if (last) {
+                acc = acc + 1 == S::kAccs ? 0 : acc + 1;
+                parity ^= acc == 0;
+                if (--left) begin();
+              }
             }
           }
-        }
+        };
+        if (__any_sync(0xFFFFFFFFu, far_scales[2 * buf] | far_scales[2 * buf + 1]))
+          add_chunk(std::true_type());
+        else
+          add_chunk(std::false_type());
         __syncwarp();
         if (lane == 0) mbar_arrive(sempty + 8 * buf);
       }
@@ -638,12 +719,15 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
           if (chunk >= 2) ok = wait_warp(sempty + 8 * buf, (chunk / 2 - 1) & 1, abort_s);
           if (!ok) break;
           float *sa = scales_a + (buf * kScaleChunk + at) * kTileM;
+          bool far = is_far(vw);
 #pragma unroll 1
           for (int r = 0; r < kTileM; r += 4 * kBatch) {
             if (r > 0) load_scales(tile, c, r);
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) sa[quarter + r + 4 * i] = v[i];
+            for (int i = 0; i < kBatch; ++i) sa[quarter + r + 4 * i] = v[i], far |= is_far(v[i]);
           }
+          far = __any_sync(0xFFFFFFFFu, far);
+          if (lane == 0) far_scales[2 * buf + warp - kScaleWarp] = far;
           if (quarter < S::kGroups) scales_w[(buf * kScaleChunk + at) * S::kGroups + quarter] = vw;
           __syncwarp();
           if (lane == 0) mbar_arrive(sfull + 8 * buf);
