@@ -123,8 +123,9 @@ int ng_pool_step_device(void *pool, const int *d_tokens, float *d_logits,
 float *ng_pool_device_state(void *pool);
 /* CUDA device the pool's sessions live on. */
 int ng_pool_device(void *pool);
-/* Reports an error that a kernel of an enqueued step recorded (a bounded wait
- * that ran out); call it after synchronising with the step's stream. */
+/* Reports an error that a kernel of this pool's enqueued steps recorded (a
+ * bounded wait that ran out), once; call it after synchronising with their
+ * stream. */
 int ng_pool_check(void *pool);
 /* Beam search: the pool's sessions in groups of `beams` (1..32, dividing the
  * pool); session w of each group takes over the state of session parents[.][w]
@@ -335,11 +336,20 @@ int ng_block_quantize(int device, const void *x, int dtype, int64_t rows, int64_
  * bytes' products of one block of 128 on the tensor cores, then the blocks in
  * a fixed order; rounded once to y's type.  Any finite scales: a block counts
  * a_scale * w_scale * its sum although the scales' product alone may leave
- * fp32's range.  The result is a function of the operands and sizes alone.  bias and add are fp32 and may be NULL; y may be
- * add when it is fp32 with the same stride. */
+ * fp32's range.  The result is a function of the operands and sizes alone, on
+ * one kind of GPU.  bias and add are fp32 and may be NULL; y may be add when it
+ * is fp32 with the same stride.
+ *
+ * A product's waits are bounded.  One that runs out (the GPU is at fault, not
+ * the operands) loses that product's result and is reported once on its device:
+ * by the next ng_block_matmul there, which then enqueues nothing, or by
+ * ng_block_check, for callers that synchronise or replay a graph and want to
+ * know.  The 8-bit projections of an engine report to the engine's and pools'
+ * own callers instead. */
 int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale, const void *w, int64_t ldw,
                     const float *w_scale, int64_t m, int64_t n, int64_t k, const float *bias, const float *add,
                     int64_t ldadd, float add_scale, void *y, int dtype, int64_t ldy, void *stream);
+int ng_block_check(int device);
 
 /* Beam search's step for `groups` searches of `beams` (1..32) beams: logits
  * [groups * beams] rows of vocab (row stride ld elements), scores [groups][beams]

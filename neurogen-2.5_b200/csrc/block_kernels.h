@@ -64,10 +64,13 @@ struct BlockMatmulArgs {
   Elem type;
   long ldy;
   int m, n, k;
+  int *err; // word to set when a wait runs out (ErrorWord::device), or null: the device's own
 };
 void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s);
-// Throws when a product on this device reported a wait that ran out since the
-// last check (its result is lost; later products run normally).
+// Throws when a product without a word of its own reported a wait that ran out
+// on this device since the last check (its result is lost; later products run
+// normally).
 void check_block_matmul_errors(int device);
+constexpr char kBlockMatmulTimeout[] = "An 8-bit product timed out waiting for its tensor-core pipeline";
 
 } // namespace ngb

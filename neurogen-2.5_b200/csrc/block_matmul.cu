@@ -18,6 +18,7 @@
 #include <climits>
 #include <cmath>
 #include <cstdlib>
+#include <memory>
 #include <mutex>
 #include <type_traits>
 
@@ -786,13 +787,12 @@ bool make_map(CUtensorMap *m, const uint8_t *p, long rows, long cols, long ld, i
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Per device: kernel attributes, SM count and the error word (pinned, mapped),
-// set up at the first call.
+// Per device: kernel attributes, SM count and the error word of products whose
+// caller brings none, set up at the first call and kept until the process ends.
 constexpr int kMaxDevices = 64;
 struct DeviceSetup {
   std::once_flag once;
-  std::atomic<int *> err{nullptr};
-  int *err_dev = nullptr;
+  std::atomic<ErrorWord *> err{nullptr};
   int sms = 0;
   int clusters[4] = {}; // clusters of 1, 2, 4 and 8 CTAs that run at once
 } g_setup[kMaxDevices];
@@ -838,11 +838,9 @@ DeviceSetup &setup() {
       cluster_config(cfg, attr, 1 << i, 1 << i, TcShape<64>::kThreads, TcShape<64>::kSmem);
       NGB_CUDA(cudaOccupancyMaxActiveClusters(&d.clusters[i], k_block_tc<64, float>, &cfg));
     }
-    int *host = nullptr;
-    NGB_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&host), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
-    *host = 0;
-    NGB_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void **>(&d.err_dev), host, 0));
-    d.err = host;
+    auto err = std::make_unique<ErrorWord>();
+    err->ensure();
+    d.err = err.release();
   });
   return d;
 }
@@ -879,8 +877,8 @@ template <int TN> void launch_tc(const BlockMatmulArgs &a, int splits, DeviceSet
   const auto kernel = a.type == Elem::f32    ? k_block_tc<TN, float>
                       : a.type == Elem::bf16 ? k_block_tc<TN, __nv_bfloat16>
                                              : k_block_tc<TN, __half>;
-  NGB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_w, a, splits, int(tiles_n), int(tiles), vector_rows(a), d.err_dev,
-                              take_stall()));
+  NGB_CUDA(cudaLaunchKernelEx(&cfg, kernel, tm_a, tm_w, a, splits, int(tiles_n), int(tiles), vector_rows(a),
+                              a.err ? a.err : d.err.load()->device(), take_stall()));
 }
 
 // The launch with the least estimated time, in microseconds.  The estimates
@@ -941,11 +939,8 @@ void preload_block_kernels() {
 
 void check_block_matmul_errors(int device) {
   if (device < 0 || device >= kMaxDevices) return;
-  int *err = g_setup[device].err;
-  if (err && *reinterpret_cast<volatile int *>(err)) {
-    *reinterpret_cast<volatile int *>(err) = 0;
-    throw std::runtime_error("An 8-bit product timed out waiting for its tensor-core pipeline");
-  }
+  const ErrorWord *err = g_setup[device].err;
+  if (err && err->take()) throw std::runtime_error(kBlockMatmulTimeout);
 }
 
 void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s) {

@@ -139,6 +139,13 @@ int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale
   });
 }
 
+int ng_block_check(int device) {
+  return guarded([&] {
+    require(device >= 0 && device < kMaxDevices, "CUDA device index out of range");
+    check_block_matmul_errors(device);
+  });
+}
+
 size_t ng_beam_workspace(int groups, int beams, int vocab) {
   if (groups < 1 || beams < 1 || beams > kMaxBeams || vocab < 1) return 0;
   return beam_workspace(groups, beams, vocab);

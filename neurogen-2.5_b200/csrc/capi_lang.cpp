@@ -212,7 +212,7 @@ int ng_pool_step(void *p, const int *tokens, float *logits, float *hidden, float
     if (activity)
       NGB_CUDA(cudaMemcpyAsync(activity, pool.act.as<float>(), size_t(B) * 4, cudaMemcpyDeviceToHost, st));
     NGB_CUDA(cudaStreamSynchronize(st));
-    m.check_device_errors();
+    m.check_device_errors(pool.sc.proj_err);
   });
 }
 
@@ -264,7 +264,9 @@ float *ng_pool_device_state(void *p) { return p ? static_cast<Pool *>(p)->state.
 int ng_pool_check(void *p) {
   return guarded([&] {
     if (!p) throw std::invalid_argument("Null pool");
-    static_cast<Pool *>(p)->engine->device().check_device_errors();
+    auto &pool = *static_cast<Pool *>(p);
+    std::lock_guard<std::mutex> lock(pool.mu);
+    pool.engine->device().check_device_errors(pool.sc.proj_err);
   });
 }
 

@@ -115,6 +115,7 @@ extern "C" int ng_step_static(void *p, int token, const float *state, size_t sta
     if (m.fp8_proj) {
       v.x_q = reinterpret_cast<uint8_t *>(base + L.x_q);
       v.x_scale = base + L.x_scale;
+      v.proj_err = m.host_scratch.proj_err.device();
     }
     float *d_state = base + L.state, *d_logits = base + L.logits, *d_hidden = base + L.hidden,
           *d_act = base + L.act;
@@ -131,6 +132,6 @@ extern "C" int ng_step_static(void *p, int token, const float *state, size_t sta
     NGB_CUDA(cudaMemcpyAsync(hidden, d_hidden, size_t(w) * sizeof(float), cudaMemcpyDeviceToHost, st));
     NGB_CUDA(cudaMemcpyAsync(activity, d_act, sizeof(float), cudaMemcpyDeviceToHost, st));
     NGB_CUDA(cudaStreamSynchronize(st));
-    m.check_device_errors(); // same error reporting as ng_step
+    m.check_device_errors(m.host_scratch.proj_err); // same error reporting as ng_step
   });
 }

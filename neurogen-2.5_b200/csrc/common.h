@@ -52,6 +52,35 @@ private:
   size_t n_ = 0;
 };
 
+// A word that a kernel sets when it gives up (pinned host memory, mapped into
+// the device), read without touching a stream.  Each caller that waits for
+// kernels of its own has one, so that it hears of its own failures and of no
+// other caller's.
+class ErrorWord {
+public:
+  ErrorWord() = default;
+  ErrorWord(const ErrorWord &) = delete;
+  ErrorWord &operator=(const ErrorWord &) = delete;
+  ~ErrorWord() {
+    if (host_) cudaFreeHost(host_);
+  }
+  void ensure() {
+    if (host_) return;
+    int *p = nullptr;
+    NGB_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&p), sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable));
+    *p = 0;
+    host_ = p;
+    NGB_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void **>(&device_), p, 0));
+  }
+  int *device() const { return device_; }
+  // Whether it has been set since the last call; one exchange, so that a
+  // setting is never lost between reading and clearing.
+  bool take() const { return host_ && __atomic_exchange_n(host_, 0, __ATOMIC_ACQ_REL) != 0; }
+
+private:
+  int *host_ = nullptr, *device_ = nullptr;
+};
+
 // Throws unless the current device is a Blackwell datacenter part (sm_100):
 // the kernels are compiled for sm_100a only and nothing else may run them.
 int require_sm100_device();

@@ -103,6 +103,7 @@ void Scratch::ensure(const LangDims &d, int batch, bool tc_proj, bool fp8_proj) 
     x_lo.reset(B * d.kmax() * 4);
   }
   if (fp8_proj) {
+    proj_err.ensure();
     x_q.reset(B * block_row_bytes(d.kmax()));
     x_scale.reset(B * scale_blocks(d.kmax()) * 4);
   }
@@ -244,27 +245,25 @@ DeviceModel::DeviceModel(const EngineConfig &cfg, const CorticalColumnV2 &col, c
   head_wr = upload(head_w, size_t(kVocab) * w);
   split_upload(head_w, size_t(kVocab) * w, head_hi, head_lo);
   head_b = upload(take(kVocab), kVocab);
-  if (fp8_proj) NGB_CUDA(cudaDeviceSynchronize()); // the weights' 8-bit forms, made on the default stream
+  if (fp8_proj) {
+    host_scratch.proj_err.ensure();    // for ng_step_static, which has no workspace of its own
+    NGB_CUDA(cudaDeviceSynchronize()); // the weights' 8-bit forms, made on the default stream
+  }
   NGB_CUDA(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
-  NGB_CUDA(cudaHostAlloc(reinterpret_cast<void **>(&readout_err), sizeof(int), cudaHostAllocMapped));
-  *readout_err = 0;
-  NGB_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void **>(&readout_err_dev), readout_err, 0));
+  readout_err.ensure();
 }
 
 DeviceModel::~DeviceModel() {
   if (stream) cudaStreamDestroy(stream);
-  if (readout_err) cudaFreeHost(readout_err);
 }
 
 // The flag is cleared as it is reported: the timed-out launch's logits are
 // lost, but the sessions' state does not depend on the readout, so the next
 // step on this engine runs normally.
-void DeviceModel::check_device_errors() const {
-  if (fp8_proj) check_block_matmul_errors(device);
-  if (readout_err && *reinterpret_cast<volatile int *>(readout_err)) {
-    *reinterpret_cast<volatile int *>(readout_err) = 0;
-    throw std::runtime_error("Readout kernel timed out waiting for its tensor-core pipeline");
-  }
+void DeviceModel::check_device_errors(const ErrorWord &proj) const {
+  const bool readout = readout_err.take();
+  if (proj.take()) throw std::runtime_error(kBlockMatmulTimeout);
+  if (readout) throw std::runtime_error("Readout kernel timed out waiting for its tensor-core pipeline");
 }
 
 void DeviceModel::enqueue_view(int B, const int *d_tokens, const float *d_inputs, bool first_idle,
@@ -278,7 +277,7 @@ void DeviceModel::enqueue_view(int B, const int *d_tokens, const float *d_inputs
   // split hidden state has somewhere to go; the sequential SIMT projection
   // otherwise.  The last LayerNorm writes the split.
   const ReadoutArgs ra{sc.h_hi, sc.h_lo, d.w, head_hi.as<float>(), head_lo.as<float>(), head_b.as<float>(),
-                       d_logits, kVocab, B, d.w, kVocab, readout_err_dev};
+                       d_logits, kVocab, B, d.w, kVocab, readout_err.device()};
   const bool tc_readout = d_logits && readout_tc_ok(ra);
   // A projection on the tensor cores (NEUROGEN_PROJECTION=tc, B >= 2): its
   // input split into tf32 hi / lo, then the readout kernel with the
@@ -292,14 +291,14 @@ void DeviceModel::enqueue_view(int B, const int *d_tokens, const float *d_inputs
       const long ldq = block_row_bytes(pa.K);
       launch_block_quantize({pa.x, Elem::f32, pa.xidx, B, pa.K, pa.ldx, 1, sc.x_q, ldq, sc.x_scale}, st);
       launch_block_matmul({sc.x_q, ldq, sc.x_scale, w_q.q.as<uint8_t>(), w_q.ld, w_q.scale.as<float>(), pa.bias, pa.addv,
-                           pa.ldadd, 0.25f, pa.y, Elem::f32, pa.ldy, B, pa.M, pa.K},
+                           pa.ldadd, 0.25f, pa.y, Elem::f32, pa.ldy, B, pa.M, pa.K, sc.proj_err},
                           st);
       return;
     }
     if (tc_proj_here) {
       launch_tf32_split(pa.x, pa.xidx, pa.ldx, pa.K, B, sc.x_hi, sc.x_lo, st);
       ReadoutArgs a{sc.x_hi, sc.x_lo, pa.K, w_hi.as<float>(), w_lo.as<float>(), pa.bias, pa.y, pa.ldy,
-                    B, pa.K, pa.M, readout_err_dev};
+                    B, pa.K, pa.M, readout_err.device()};
       a.addv = pa.addv;
       a.ldadd = pa.ldadd;
       if (launch_readout_tc(a, st)) return;
@@ -540,7 +539,7 @@ void NeuralEngine::step_batch(const int *tokens, int batch, const float *state, 
   if (activity)
     NGB_CUDA(cudaMemcpyAsync(activity, sc.act.as<float>(), size_t(batch) * 4, cudaMemcpyDeviceToHost, st));
   NGB_CUDA(cudaStreamSynchronize(st));
-  m.check_device_errors();
+  m.check_device_errors(sc.proj_err);
 }
 
 void NeuralEngine::advance_batch(const float *inputs, int batch, const float *state, bool idle,
@@ -565,7 +564,7 @@ void NeuralEngine::advance_batch(const float *inputs, int batch, const float *st
   if (activity)
     NGB_CUDA(cudaMemcpyAsync(activity, sc.act.as<float>(), size_t(batch) * 4, cudaMemcpyDeviceToHost, st));
   NGB_CUDA(cudaStreamSynchronize(st));
-  m.check_device_errors();
+  m.check_device_errors(sc.proj_err);
 }
 
 Vector NeuralEngine::step(int token, std::vector<ColumnState> &state, Vector &hidden, float &activity) {

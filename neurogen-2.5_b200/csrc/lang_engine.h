@@ -53,6 +53,7 @@ struct ScratchView {
   float *x_hi = nullptr, *x_lo = nullptr; // [B][max K] tf32 split of a projection's input, or null
   uint8_t *x_q = nullptr;                 // [B][max K, to 16] 8-bit input of a projection, or null
   float *x_scale = nullptr;               // [B][ceil(max K / 128)] its scales, or null
+  int *proj_err = nullptr;                // set when an 8-bit projection gives up, or null
 };
 
 // Per-call device workspace for `capacity` sessions.
@@ -60,11 +61,12 @@ struct Scratch {
   int capacity = 0;
   DeviceBuffer h, hraw, vin, fb, tr, feat, cnt, tokens, inputs, state, logits, hidden, act, h_hi, h_lo, x_hi, x_lo,
       x_q, x_scale;
+  ErrorWord proj_err; // of the 8-bit projections that use this workspace
   void ensure(const LangDims &d, int batch, bool tc_proj, bool fp8_proj);
   ScratchView view() const {
     return {h.as<float>(),   hraw.as<float>(), vin.as<float>(),  fb.as<float>(),  tr.as<float>(),
             feat.as<float>(), cnt.as<int>(),    h_hi.as<float>(), h_lo.as<float>(), x_hi.as<float>(),
-            x_lo.as<float>(), x_q.as<uint8_t>(), x_scale.as<float>()};
+            x_lo.as<float>(), x_q.as<uint8_t>(), x_scale.as<float>(), proj_err.device()};
   }
 };
 
@@ -109,11 +111,10 @@ public:
   bool fp8_proj = false;
   std::vector<RegionWeights> regions;
   Scratch host_scratch; // used by the host-buffer entry points (under the engine mutex)
-  // Error word of the tensor-core readout (pinned, mapped into the device):
-  // nonzero after one of its bounded waits timed out.
-  int *readout_err = nullptr, *readout_err_dev = nullptr;
-  // Throws when a kernel reported an error; call after synchronising.
-  void check_device_errors() const;
+  ErrorWord readout_err; // of the tensor-core readout: set after one of its bounded waits ran out
+  // Throws when a kernel reported an error: the readout of this engine, or an
+  // 8-bit projection to `proj`, its workspace's word.  Call after synchronising.
+  void check_device_errors(const ErrorWord &proj) const;
 };
 
 } // namespace ngb

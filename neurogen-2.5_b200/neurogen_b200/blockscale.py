@@ -102,6 +102,15 @@ def matmul(a, a_scale, w, w_scale, bias=None, add=None, add_scale=1.0, out_dtype
     return y
 
 
+def check_products(device=None):
+    """Raise ValueError when a product on ``device`` (default: the current one) has given up a wait since
+    the last call that reported one; synchronise before.  ``matmul`` asks the same before it starts:
+    this is for callers that replay a graph or have no further product to make.
+    """
+    index = None if device is None else torch.device(device).index
+    check(library().ng_block_check(torch.cuda.current_device() if index is None else index))
+
+
 def linear(x, w, w_scale, bias=None, add=None, add_scale=1.0, out_dtype=torch.float32):
     """``quantize(x)`` times the block-scaled weights ``w``: a projection in 8 bits."""
     return matmul(*quantize(x), w, w_scale, bias, add, add_scale, out_dtype)

@@ -1,0 +1,103 @@
+"""A tensor-core product whose bounded wait runs out: who hears of it.
+
+The test switch (NEUROGEN_TEST_MATMUL_STALL=1) makes the process's first tensor-core product take the
+path of a wait that ran out, before it issues any copy or MMA, so each case is a process of its own.
+A pool's step is captured at its first use, the switched product with it.
+"""
+import os
+import subprocess
+import sys
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+SETUP = r'''
+import sys
+sys.path[:0] = {paths!r}
+import numpy as np, torch
+from neurogen_b200 import blockscale
+from neurogen_b200.language import LanguageConfig, NativeLanguageModel, SessionPool, init_packed_weights
+TIMEOUT = 'An 8-bit product timed out'
+
+def error_of(call):
+    try:
+        call()
+    except ValueError as e:
+        return str(e)
+    return ''
+
+def product(m=400, n=4096, k=512):
+    gen = torch.Generator('cuda').manual_seed(1)
+    a, sa = blockscale.quantize(torch.randn((m, k), generator=gen, device='cuda'))
+    w, sw = blockscale.quantize(torch.randn((n, k), generator=gen, device='cuda'), 128)
+    x = a.double() * sa.double().repeat_interleave(128, 1)
+    z = w.double() * sw.double().repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)
+    return (a, sa, w, sw), x @ z.T
+
+def right(y, want):   # (128 + 4 + 4) 2^-23 of the sum of magnitudes, below 512 * 0.64 * 3
+    return bool(((y.double() - want).abs() < 136 * 2.0 ** -23 * 1000).all())
+
+def model():   # sizes whose projections of 256 sessions go to the tensor cores
+    cfg = LanguageConfig(columns=32, width=768, regions=1, ticks=1, idle_steps=0)
+    return NativeLanguageModel(cfg, init_packed_weights(cfg, seed=0))
+
+def device_step(pool, stream):
+    tokens = torch.full((pool.sessions,), 5, dtype=torch.int32, device='cuda')
+    torch.cuda.synchronize()
+    assert pool.lib.ng_pool_step_device(pool.h, tokens.data_ptr(), None, stream.cuda_stream) == 0, pool.lib.ng_error()
+    stream.synchronize()
+'''
+
+
+def run(tmp_path, body):
+    script = tmp_path / 'child.py'
+    script.write_text(SETUP.format(paths=[str(p) for p in sys.path[:3]]) + body + "\nprint('done')\n")
+    env = dict(os.environ, NEUROGEN_TEST_MATMUL_STALL='1', NEUROGEN_PROJECTION='fp8')
+    out = subprocess.run([sys.executable, str(script)], env=env, capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and out.stdout.endswith('done\n'), out.stdout + out.stderr[-3000:]
+
+
+def test_a_standalone_product_is_asked_for_by_itself(tmp_path):
+    """Without a further product, and once."""
+    run(tmp_path, r'''
+ops, want = product()
+blockscale.check_products()
+blockscale.matmul(*ops)
+torch.cuda.synchronize()
+assert TIMEOUT in error_of(blockscale.check_products)
+blockscale.check_products('cuda:0')
+assert right(blockscale.matmul(*ops), want)
+''')
+
+
+def test_a_pool_hears_of_its_own_products_only(tmp_path):
+    """A standalone product, another pool and a host batch of the same engine run between the failure and
+    the pool's check: none of them is refused or blamed, and the pool is told."""
+    run(tmp_path, r'''
+mod = model()
+lost, other, stream = SessionPool(mod, 256), SessionPool(mod, 256), torch.cuda.Stream()
+device_step(lost, stream)
+ops, want = product()
+assert right(blockscale.matmul(*ops), want)
+blockscale.check_products()
+tokens = np.full(256, 5)
+logits = other.step(tokens)
+state = np.zeros((256, mod.engine.state_size), np.float32)
+assert np.array_equal(mod.engine.step_batch(tokens, state)[0], logits)
+assert TIMEOUT in error_of(lambda: lost._check(lost.lib.ng_pool_check(lost.h)))
+other._check(other.lib.ng_pool_check(other.h))
+assert np.isfinite(other.step(tokens)).all()
+''')
+
+
+def test_a_host_batch_reports_its_own_product(tmp_path):
+    run(tmp_path, r'''
+mod = model()
+tokens, state = np.full(256, 5), np.zeros((256, mod.engine.state_size), np.float32)
+assert TIMEOUT in error_of(lambda: mod.engine.step_batch(tokens, state))
+logits = mod.engine.step_batch(tokens, state)[0]
+pool = SessionPool(mod, 256)
+assert np.array_equal(pool.step(tokens), logits)
+blockscale.check_products()
+''')
