@@ -341,7 +341,8 @@ int ng_block_quantize(int device, const void *x, int dtype, int64_t rows, int64_
  * is fp32 with the same stride.
  *
  * A product's waits are bounded.  One that runs out (the GPU is at fault, not
- * the operands) loses that product's result and is reported once on its device:
+ * the operands) loses that product's result, whose lost elements read NaN, and
+ * is reported once on its device:
  * by the next ng_block_matmul there, which then enqueues nothing, or by
  * ng_block_check, for callers that synchronise or replay a graph and want to
  * know.  The 8-bit projections of an engine report to the engine's and pools'

@@ -227,8 +227,13 @@ __global__ void __launch_bounds__(32 * kVecWarps, CTAS) k_block_vec(BlockMatmulA
 // each owns a slice of the rows, all send it their sums of these rows
 // (distributed shared memory), and it adds them up in rank order.
 //
-// Every wait is bounded.  One that runs out sets *err; its role stops, waits
-// (bounded) for its own copies or MMAs in flight, and the CTA frees its TMEM.
+// Every wait on an mbarrier is bounded.  One that runs out sets *err; its role
+// stops, waits (bounded) for its own copies or MMAs in flight, and the CTA
+// frees its TMEM and fills its part of the result with NaN.  The cluster's
+// barriers and the TMEM allocation have no limit of their own and need none:
+// every role of every CTA reaches each barrier, whether its waits ran out or
+// not, and TMEM is held only by CTAs that run to their end without this one
+// (of a cluster of this kernel an SM holds one CTA, so none waits for another's).
 constexpr int kTileM = 128;       // rows of a in a tile
 constexpr int kMaxSplits = 8;
 constexpr int kScaleChunk = 16;   // blocks along k whose scales are staged at a time (two such buffers)
@@ -744,11 +749,14 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
   }
   fence_before();
   __syncthreads();
-  const bool failed = *abort_s != 0;
+  bool failed = *abort_s != 0;
   if (failed && tid == 0) *reinterpret_cast<volatile int *>(err) = 1;
   if (splits > 1) {
+    // Rows of the cluster's other CTAs lack a failed one's sums: they fail with it.
+    if (failed && tid < splits) *cg::this_cluster().map_shared_rank(const_cast<int *>(abort_s), tid) = 1;
     cluster_arrive();
     cluster_wait(); // every CTA has sent its sums
+    failed = *abort_s != 0;
     if (!failed) {
       const int n0 = first % tiles_n * TN, rows = kTileM / splits, m0 = first / tiles_n * kTileM + z * rows;
       const int valid = min(rows, a.m - m0);
@@ -765,6 +773,16 @@ __global__ void __launch_bounds__(TcShape<TN>::kThreads, 1)
             v.x = __fadd_rn(v.x, x[s].x), v.y = __fadd_rn(v.y, x[s].y), v.z = __fadd_rn(v.z, x[s].z), v.w = __fadd_rn(v.w, x[s].w);
         store4<Y>(a, m0 + r, n0 + 4 * j, v, vec);
       }
+    }
+  }
+  // A lost result reads NaN, not what its memory held before.
+  if (failed) {
+    const int rows = kTileM / splits;
+    for (int tile = first; tile < tiles; tile += stride) {
+      const int m0 = tile / tiles_n * kTileM + (splits > 1 ? z * rows : 0), n0 = tile % tiles_n * TN;
+      for (int i = tid; i < rows * TN; i += S::kThreads)
+        if (m0 + i / TN < a.m && n0 + i % TN < a.n)
+          store_elem(a.y, a.type, long(m0 + i / TN) * a.ldy + n0 + i % TN, __int_as_float(0x7FFFFFFF));
     }
   }
   if (warp == kMmaWarp) {

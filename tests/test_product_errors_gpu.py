@@ -101,3 +101,26 @@ pool = SessionPool(mod, 256)
 assert np.array_equal(pool.step(tokens), logits)
 blockscale.check_products()
 ''')
+
+
+@pytest.mark.parametrize('m,n,k', [(35, 2810, 150), (35, 1374, 3293), (304, 124, 4364), (277, 3297, 145), (563, 4070, 141)])
+@pytest.mark.parametrize('code,dtype', [(0, 'float32'), (1, 'bfloat16'), (2, 'float16')])
+def test_a_lost_result_reads_nan(tmp_path, m, n, k, code, dtype):
+    """Tiles walked over and k ranges shared by a cluster; nothing beside or behind the result is written."""
+    run(tmp_path, rf'''
+m, n, k = {m}, {n}, {k}
+from neurogen_b200 import library
+a, sa = blockscale.quantize(torch.randn((m, k), device='cuda'))
+w, sw = blockscale.quantize(torch.randn((n, k), device='cuda'), 128)
+y = torch.full((m + 3, n + 5), 3.5, dtype=torch.{dtype}, device='cuda')
+stream = torch.cuda.current_stream().cuda_stream
+for lost in (True, False):
+    code = library().ng_block_matmul(0, a.data_ptr(), a.stride(0), sa.data_ptr(), w.data_ptr(), w.stride(0), sw.data_ptr(),
+                                     m, n, k, None, None, n, 1.0, y.data_ptr(), {code}, n + 5, stream)
+    assert code == 0, library().ng_error()
+    assert (torch.isnan if lost else torch.isfinite)(y[:m, :n]).all()
+    assert (y[m:] == 3.5).all() and (y[:, n:] == 3.5).all()
+    if lost:
+        torch.cuda.synchronize()
+        assert TIMEOUT in error_of(blockscale.check_products)
+''')
