@@ -108,7 +108,8 @@ int ng_math_eval(const float *x, size_t n, float *tanh_out, float *sigmoid_out);
  * zero-initialised (the reference model's initial state, model.py:68-70). */
 void *ng_pool_create(void *engine, int batch);
 void ng_pool_destroy(void *pool);
-/* Copy all session states in/out, host layout [batch, state_size]. */
+/* Copy all session states in/out, host layout [batch, state_size], after the
+ * steps on the engine's stream (synchronise a stream of your own first). */
 int ng_pool_load(void *pool, const float *state);
 int ng_pool_store(void *pool, float *state);
 /* One token per session: tokens [batch] (host), logits [batch, 264] (host,
@@ -124,8 +125,11 @@ float *ng_pool_device_state(void *pool);
 /* CUDA device the pool's sessions live on. */
 int ng_pool_device(void *pool);
 /* Reports an error that a kernel of this pool's enqueued steps recorded (a
- * bounded wait that ran out), once; call it after synchronising with their
- * stream. */
+ * bounded wait that ran out); call it after synchronising with their stream.
+ * After a readout that timed out the step's logits are lost and the pool goes
+ * on.  After an 8-bit projection that did, the states that the step advanced
+ * are lost: this call, the steps, the reorderings and ng_pool_store all fail
+ * until ng_pool_load has replaced them. */
 int ng_pool_check(void *pool);
 /* Beam search: the pool's sessions in groups of `beams` (1..32, dividing the
  * pool); session w of each group takes over the state of session parents[.][w]

@@ -33,10 +33,36 @@ struct Pool {
   Scratch sc;
   cudaStream_t stream = nullptr;
   cudaGraphExec_t graph = nullptr; // one token step of the whole pool
+  bool lost = false;               // a step's projection failed: the states are not to be used
   std::mutex mu;
   ~Pool() {
     if (graph) cudaGraphExecDestroy(graph);
     if (stream) cudaStreamDestroy(stream);
+  }
+  // Reports errors of the steps that have run so far.
+  void check_errors() {
+    try {
+      engine->device().check_device_errors(sc.proj_err);
+    } catch (const ProjectionLost &) {
+      lost = true;
+      throw;
+    }
+  }
+  // Before the states are used.  A step still running may fail later; what has
+  // been reported to the host by now is heard here.
+  void require_states() {
+    if (sc.proj_err.take()) lost = true;
+    if (lost)
+      throw std::runtime_error("The pool's states are lost (an 8-bit projection timed out); load states before going on");
+  }
+  // The states have been replaced and nothing of the pool is running: it starts afresh.
+  void found() {
+    (void)sc.proj_err.take();
+    if (lost && graph) {
+      cudaGraphExecDestroy(graph);
+      graph = nullptr;
+    }
+    lost = false;
   }
   // Enqueue one token step reading `tokens` and writing logits/hidden/act
   // into the pool's own buffers.  The step is captured into a CUDA graph on
@@ -176,7 +202,9 @@ int ng_pool_load(void *p, const float *state) {
     for (size_t i = 0; i < count; ++i)
       if (!std::isfinite(state[i])) throw std::invalid_argument("Non-finite native state");
     NGB_CUDA(cudaSetDevice(pool.engine->device().device));
+    NGB_CUDA(cudaStreamSynchronize(pool.stream));
     NGB_CUDA(cudaMemcpy(pool.state.as<float>(), state, count * 4, cudaMemcpyHostToDevice));
+    pool.found();
   });
 }
 
@@ -187,6 +215,7 @@ int ng_pool_store(void *p, float *state) {
     std::lock_guard<std::mutex> lock(pool.mu);
     NGB_CUDA(cudaSetDevice(pool.engine->device().device));
     NGB_CUDA(cudaStreamSynchronize(pool.stream));
+    pool.require_states();
     NGB_CUDA(cudaMemcpy(state, pool.state.as<float>(), pool.engine->state_size() * pool.B * 4,
                         cudaMemcpyDeviceToHost));
   });
@@ -199,8 +228,8 @@ int ng_pool_step(void *p, const int *tokens, float *logits, float *hidden, float
     std::lock_guard<std::mutex> lock(pool.mu);
     for (int b = 0; b < pool.B; ++b)
       if (tokens[b] < 0 || tokens[b] >= kVocab) throw std::invalid_argument("Token must be in 0..263");
-    DeviceModel &m = pool.engine->device();
-    NGB_CUDA(cudaSetDevice(m.device));
+    pool.require_states();
+    NGB_CUDA(cudaSetDevice(pool.engine->device().device));
     cudaStream_t st = pool.stream;
     const int B = pool.B, w = pool.engine->config.width;
     NGB_CUDA(cudaMemcpyAsync(pool.tokens.as<int>(), tokens, B * sizeof(int), cudaMemcpyHostToDevice, st));
@@ -212,7 +241,7 @@ int ng_pool_step(void *p, const int *tokens, float *logits, float *hidden, float
     if (activity)
       NGB_CUDA(cudaMemcpyAsync(activity, pool.act.as<float>(), size_t(B) * 4, cudaMemcpyDeviceToHost, st));
     NGB_CUDA(cudaStreamSynchronize(st));
-    m.check_device_errors(pool.sc.proj_err);
+    pool.check_errors();
   });
 }
 
@@ -221,8 +250,8 @@ int ng_pool_step_device(void *p, const int *d_tokens, float *d_logits, void *str
     if (!p || !d_tokens) throw std::invalid_argument("Null pool or tokens");
     auto &pool = *static_cast<Pool *>(p);
     std::lock_guard<std::mutex> lock(pool.mu);
-    DeviceModel &m = pool.engine->device();
-    NGB_CUDA(cudaSetDevice(m.device));
+    pool.require_states();
+    NGB_CUDA(cudaSetDevice(pool.engine->device().device));
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : pool.stream;
     NGB_CUDA(cudaMemcpyAsync(pool.tokens.as<int>(), d_tokens, pool.B * sizeof(int), cudaMemcpyDeviceToDevice, st));
     pool.token_step(st);
@@ -240,6 +269,7 @@ int ng_pool_reorder(void *p, int beams, const int32_t *parents) {
     pool.check_beams(beams);
     for (int b = 0; b < pool.B; ++b)
       if (parents[b] < 0 || parents[b] >= beams) throw std::invalid_argument("Parents must be beams of the same group");
+    pool.require_states();
     NGB_CUDA(cudaSetDevice(pool.engine->device().device));
     NGB_CUDA(cudaMemcpyAsync(pool.parents.as<int>(), parents, pool.B * sizeof(int), cudaMemcpyHostToDevice,
                              pool.stream));
@@ -254,6 +284,7 @@ int ng_pool_reorder_device(void *p, int beams, const int32_t *d_parents, void *s
     auto &pool = *static_cast<Pool *>(p);
     std::lock_guard<std::mutex> lock(pool.mu);
     pool.check_beams(beams);
+    pool.require_states();
     NGB_CUDA(cudaSetDevice(pool.engine->device().device));
     pool.reorder(beams, d_parents, stream ? static_cast<cudaStream_t>(stream) : pool.stream);
   });
@@ -266,7 +297,8 @@ int ng_pool_check(void *p) {
     if (!p) throw std::invalid_argument("Null pool");
     auto &pool = *static_cast<Pool *>(p);
     std::lock_guard<std::mutex> lock(pool.mu);
-    pool.engine->device().check_device_errors(pool.sc.proj_err);
+    pool.check_errors();
+    pool.require_states();
   });
 }
 

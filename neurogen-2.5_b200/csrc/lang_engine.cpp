@@ -257,12 +257,13 @@ DeviceModel::~DeviceModel() {
   if (stream) cudaStreamDestroy(stream);
 }
 
-// The flag is cleared as it is reported: the timed-out launch's logits are
-// lost, but the sessions' state does not depend on the readout, so the next
-// step on this engine runs normally.
+// A word is cleared as it is reported.  After a readout that timed out the
+// launch's logits are lost, but the sessions' states do not depend on it, so
+// the next step runs normally.  A projection does feed the states: a caller that
+// keeps them on the device must not go on with them.
 void DeviceModel::check_device_errors(const ErrorWord &proj) const {
   const bool readout = readout_err.take();
-  if (proj.take()) throw std::runtime_error(kBlockMatmulTimeout);
+  if (proj.take()) throw ProjectionLost(kBlockMatmulTimeout);
   if (readout) throw std::runtime_error("Readout kernel timed out waiting for its tensor-core pipeline");
 }
 

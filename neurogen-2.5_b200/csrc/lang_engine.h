@@ -70,6 +70,11 @@ struct Scratch {
   }
 };
 
+// An 8-bit projection gave up: the states that its step advanced are lost.
+struct ProjectionLost : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+
 class DeviceModel {
 public:
   DeviceModel(const neurogen::cortical::EngineConfig &cfg,
@@ -113,7 +118,8 @@ public:
   Scratch host_scratch; // used by the host-buffer entry points (under the engine mutex)
   ErrorWord readout_err; // of the tensor-core readout: set after one of its bounded waits ran out
   // Throws when a kernel reported an error: the readout of this engine, or an
-  // 8-bit projection to `proj`, its workspace's word.  Call after synchronising.
+  // 8-bit projection to `proj`, its workspace's word (ProjectionLost).  Call
+  // after synchronising.
   void check_device_errors(const ErrorWord &proj) const;
 };
 

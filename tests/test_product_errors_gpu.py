@@ -124,3 +124,39 @@ for lost in (True, False):
         torch.cuda.synchronize()
         assert TIMEOUT in error_of(blockscale.check_products)
 ''')
+
+
+@pytest.mark.parametrize('host', [True, False])
+def test_a_pool_whose_projection_was_lost_refuses_its_states(tmp_path, host):
+    """A projection feeds the states, in place: after one that gave up nothing uses them until they are
+    set again, and then the pool steps as a fresh one does.  Another pool of the engine is not affected."""
+    run(tmp_path, f'HOST = {host}' + r'''
+mod = model()
+pool, other = SessionPool(mod, 256), SessionPool(mod, 256)
+start = np.random.default_rng(0).uniform(0, 0.4, (256, mod.engine.state_size)).astype(np.float32)
+pool.set_states(start)
+other.set_states(start)
+tokens = np.full(256, 5)
+if HOST:
+    assert TIMEOUT in error_of(lambda: pool.step(tokens))
+else:
+    device_step(pool, torch.cuda.Stream())
+    assert 'lost' in error_of(lambda: pool.step(tokens))   # heard before another step is enqueued
+logits = other.step(tokens)
+parents = np.zeros((64, 4), np.int32)
+d_parents = torch.zeros((64, 4), dtype=torch.int32, device='cuda')
+d_tokens = torch.full((256,), 5, dtype=torch.int32, device='cuda')
+for call in (lambda: pool.step(tokens), pool.states, lambda: pool.reorder(4, parents),
+             lambda: pool.beam_search(np.full((64, 1), 5), 4, 2),
+             lambda: pool._check(pool.lib.ng_pool_step_device(pool.h, d_tokens.data_ptr(), None, None)),
+             lambda: pool._check(pool.lib.ng_pool_reorder_device(pool.h, 4, d_parents.data_ptr(), None)),
+             lambda: pool._check(pool.lib.ng_pool_check(pool.h))):
+    message = error_of(call)
+    assert 'states are lost' in message and 'load states' in message, message
+assert error_of(lambda: pool.set_states(np.full_like(start, np.nan))) and 'lost' in error_of(pool.states)
+pool.set_states(start)
+assert np.array_equal(pool.states(), start)
+assert np.array_equal(pool.step(tokens), logits)
+pool._check(pool.lib.ng_pool_check(pool.h))
+assert np.array_equal(pool.states(), other.states())
+''')
