@@ -492,8 +492,9 @@ class SessionPool:
         best first: the cumulative log probability of the chosen tokens, over the tokens that
         ``allowed`` (bool [264], default every byte and control token) admits.  A beam that has
         chosen ``end`` is finished and continues with PAD at its score.  Afterwards each session has
-        been fed its own sequence, and ``logits`` holds its next logits.  The loop runs on the device
-        (token step, selection, reordering of states); tokens come back once, at the end.
+        been fed its own sequence, and ``logits`` holds its next logits; after an exception the sessions
+        are somewhere on the way there.  The loop runs on the device (token step, selection, reordering of
+        states); tokens come back once, at the end.
         """
         from . import decoding
         prompts = np.ascontiguousarray(prompts, dtype=np.int64)
@@ -516,33 +517,36 @@ class SessionPool:
         # A stream of its own: the pool's calls take the default stream's handle, 0, for the engine's stream.
         side = torch.cuda.Stream(device)
         side.wait_stream(torch.cuda.current_stream(device))
-        with torch.cuda.device(device), torch.cuda.stream(side):
-            stream = side.cuda_stream
-            logits = torch.empty((self.sessions, VOCAB), device=device)
-            feed = torch.from_numpy(prompts.T.astype(np.int32)).to(device).repeat_interleave(beams, 1)
-            if allowed is not None:
-                allowed = allowed.to(device).contiguous()
-            first = torch.zeros((groups, beams), dtype=torch.int32, device=device)
-            self._check(self.lib.ng_pool_reorder_device(self.h, beams, first.data_ptr(), stream))
+        try:
+            with torch.cuda.device(device), torch.cuda.stream(side):
+                stream = side.cuda_stream
+                logits = torch.empty((self.sessions, VOCAB), device=device)
+                feed = torch.from_numpy(prompts.T.astype(np.int32)).to(device).repeat_interleave(beams, 1)
+                if allowed is not None:
+                    allowed = allowed.to(device).contiguous()
+                first = torch.zeros((groups, beams), dtype=torch.int32, device=device)
+                self._check(self.lib.ng_pool_reorder_device(self.h, beams, first.data_ptr(), stream))
 
-            def step(tokens):
-                self._check(self.lib.ng_pool_step_device(self.h, tokens.data_ptr(), logits.data_ptr(), stream))
+                def step(tokens):
+                    self._check(self.lib.ng_pool_step_device(self.h, tokens.data_ptr(), logits.data_ptr(), stream))
 
-            for row in feed:
-                step(row)
-            scores = torch.full((groups, beams), -float('inf'), device=device)
-            scores[:, 0] = 0
-            finished = torch.zeros((groups, beams), dtype=torch.bool, device=device)
-            chosen = []
-            for _ in range(steps):
-                scores, tokens, parents, finished = decoding.beam_select(logits, scores, finished, allowed, end, PAD)
-                self._check(self.lib.ng_pool_reorder_device(self.h, beams, parents.data_ptr(), stream))
-                step(tokens)
-                chosen.append((tokens, parents))
-            tokens = torch.stack([t for t, _ in chosen]).cpu().numpy()
-            parents = torch.stack([p for _, p in chosen]).cpu().numpy()
-            scores = scores.cpu().numpy()
-            self.logits = logits.cpu().numpy()
+                for row in feed:
+                    step(row)
+                scores = torch.full((groups, beams), -float('inf'), device=device)
+                scores[:, 0] = 0
+                finished = torch.zeros((groups, beams), dtype=torch.bool, device=device)
+                chosen = []
+                for _ in range(steps):
+                    scores, tokens, parents, finished = decoding.beam_select(logits, scores, finished, allowed, end, PAD)
+                    self._check(self.lib.ng_pool_reorder_device(self.h, beams, parents.data_ptr(), stream))
+                    step(tokens)
+                    chosen.append((tokens, parents))
+                tokens = torch.stack([t for t, _ in chosen]).cpu().numpy()
+                parents = torch.stack([p for _, p in chosen]).cpu().numpy()
+                scores = scores.cpu().numpy()
+                self.logits = logits.cpu().numpy()
+        finally:   # an exception too leaves nothing of the search running: the pool's other calls use another stream
+            side.synchronize()
         self._check(self.lib.ng_pool_check(self.h))
         return trace_beams(tokens, parents), scores
 
