@@ -356,6 +356,13 @@ int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale
                     int64_t ldadd, float add_scale, void *y, int dtype, int64_t ldy, void *stream);
 int ng_block_check(int device);
 
+/* Which launch a product of this size takes (like ng_net_launch_kind, for tests
+ * and tuning): 8, 16 or 32 for the few-row kernel with so many rows of a a CTA;
+ * 1000 * columns + CTAs for the tensor-core kernel with tiles of so many columns
+ * (32, 64, 128, 256), each tile's k range shared by so many CTAs (1, 2, 4, 8);
+ * -1 on error. */
+int ng_block_matmul_kind(int device, int64_t m, int64_t n, int64_t k);
+
 /* Beam search's step for `groups` searches of `beams` (1..32) beams: logits
  * [groups * beams] rows of vocab (row stride ld elements), scores [groups][beams]
  * the beams' cumulative log probabilities (-inf: no such beam), finished

@@ -67,6 +67,11 @@ struct BlockMatmulArgs {
   int *err; // word to set when a wait runs out (ErrorWord::device), or null: the device's own
 };
 void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s);
+// Which launch a product of this size takes on the current device: 8, 16 or 32
+// for the few-row kernel with so many rows of a a CTA, 1000 * columns + CTAs
+// for the tensor-core kernel with tiles of so many columns, each tile's k range
+// shared by so many CTAs.
+int block_matmul_kind(int m, int n, int k);
 // Throws when a product without a word of its own reported a wait that ran out
 // on this device since the last check (its result is lost; later products run
 // normally).

@@ -961,6 +961,13 @@ void check_block_matmul_errors(int device) {
   if (err && err->take()) throw std::runtime_error(kBlockMatmulTimeout);
 }
 
+int block_matmul_kind(int m, int n, int k) {
+  BlockMatmulArgs a{};
+  a.m = m, a.n = n, a.k = k;
+  const Plan p = plan(a, setup());
+  return p.vec ? 8 * p.vec : 1000 * p.tn + p.splits;
+}
+
 void launch_block_matmul(const BlockMatmulArgs &a, cudaStream_t s) {
   DeviceSetup &d = setup();
   const Plan p = plan(a, d);

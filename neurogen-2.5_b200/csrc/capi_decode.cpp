@@ -139,6 +139,17 @@ int ng_block_matmul(int device, const void *a, int64_t lda, const float *a_scale
   });
 }
 
+int ng_block_matmul_kind(int device, int64_t m, int64_t n, int64_t k) {
+  int kind = 0;
+  const int code = guarded([&] {
+    require(m >= 1 && m <= INT_MAX / 2 && n >= 1 && n <= INT_MAX / 2 && k >= 1 && k <= INT_MAX / 2,
+            "Matrix size out of range");
+    OnDevice on(device);
+    kind = block_matmul_kind(int(m), int(n), int(k));
+  });
+  return code ? code : kind;
+}
+
 int ng_block_check(int device) {
   return guarded([&] {
     require(device >= 0 && device < kMaxDevices, "CUDA device index out of range");

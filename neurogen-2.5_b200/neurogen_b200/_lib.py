@@ -31,8 +31,8 @@ EXPORTS = (
     'ng_topology_export', 'ng_net_create_topology', 'ng_net_stats', 'ng_step_static', 'ng_net_launch_kind',
     'ng_net_create_partitioned', 'ng_nccl_unique_id', 'ng_math_eval', 'ng_net_plasticity_state',
     'ng_net_exchange_kind', 'ng_pool_reorder', 'ng_pool_reorder_device', 'ng_pool_device', 'ng_pool_check',
-    'ng_block_quantize', 'ng_block_matmul', 'ng_block_check', 'ng_beam_workspace', 'ng_beam_select',
-    'ng_state_reorder',
+    'ng_block_quantize', 'ng_block_matmul', 'ng_block_check', 'ng_block_matmul_kind',
+    'ng_beam_workspace', 'ng_beam_select', 'ng_state_reorder',
 )
 
 
@@ -128,6 +128,8 @@ def library():
     lib.ng_block_matmul.restype = ci
     lib.ng_block_check.argtypes = [ci]
     lib.ng_block_check.restype = ci
+    lib.ng_block_matmul_kind.argtypes = [ci, i64, i64, i64]
+    lib.ng_block_matmul_kind.restype = ci
     lib.ng_beam_workspace.argtypes = [ci, ci, ci]
     lib.ng_beam_workspace.restype = sz
     lib.ng_beam_select.argtypes = [ci, vp, ci, i64, ci, ci, ci, vp, vp, vp, ci, ci, vp, vp, vp, vp, vp, sz, vp]
