@@ -317,8 +317,10 @@ int ng_net_run_device(void *net, int ticks, uint32_t *d_spikes,
 /* Every call takes the device its arrays live on and a stream of that device
  * (cudaStream_t as void*; NULL = the default stream), enqueues its work there,
  * and returns without synchronising; the caller's current device stays as it
- * is.  Nothing is allocated, and nothing is kept between calls.  Calls can be
- * captured into CUDA graphs once the same call has run outside one. */
+ * is.  The first product on a device sets its kernels up there (and allocates
+ * the word of ng_block_check); nothing else is allocated, and of a call's data
+ * nothing is kept.  Calls can be captured into CUDA graphs once the same call
+ * has run outside one. */
 
 /* Element types of 16- and 32-bit arrays. */
 enum { NG_F32 = 0, NG_BF16 = 1, NG_F16 = 2 };
@@ -327,6 +329,8 @@ enum { NG_F32 = 0, NG_BF16 = 1, NG_F16 = 2 };
  * 128 columns and block_rows rows (1: activations, 128: weights), scales
  * row-major [ceil(rows / block_rows)][ceil(cols / 128)]; a value stands for
  * byte * scale.  8-bit rows start on 16-byte boundaries (address and stride).
+ * Rows are read in aligned words of 16 bytes: bytes beside a row in the words of
+ * its ends are read too, and not used.
  *
  * scale = max(amax |x| / 448, 2^-126), byte = e4m3(x / scale), both divisions
  * rounded to fp32 and the byte to nearest even.  A block with a NaN has a NaN
@@ -341,7 +345,7 @@ int ng_block_quantize(int device, const void *x, int dtype, int64_t rows, int64_
  * a fixed order; rounded once to y's type.  Any finite scales: a block counts
  * a_scale * w_scale * its sum although the scales' product alone may leave
  * fp32's range.  The result is a function of the operands and sizes alone, on
- * one kind of GPU.  bias and add are fp32 and may be NULL; y may be add when it
+ * one GPU.  bias and add are fp32 and may be NULL; y may be add when it
  * is fp32 with the same stride.
  *
  * A product's waits are bounded.  One that runs out (the GPU is at fault, not
@@ -373,13 +377,15 @@ int ng_block_matmul_kind(int device, int64_t m, int64_t n, int64_t k);
  * `pad` at its own score.  The best `beams` candidates, best first, become
  * next_scores, tokens, parents (the beam within the group) and next_finished
  * (the parent's, or the token is `end`; end < 0: no token ends a beam).  Scores
- * are formed in 64 bits and rounded once; a beam's equal logits go to the lower
- * token, equal 64-bit scores of two beams to the lower beam (rows that hold the
- * same values in another order have sums that may differ in their last bits).
- * A candidate whose score
- * is not finite is none (a row whose mask leaves nothing, or that holds a NaN
- * or +inf at an allowed token, has none); slots that no candidate fills get
- * score -inf, `pad`, their own index as parent, and count as finished.
+ * are formed in 64 bits, from exponentials good to 1e-12 of their value, and
+ * rounded once.  A beam's equal logits go to the lower token, which no
+ * arithmetic decides.  Equal 64-bit scores of two beams go to the lower beam:
+ * two beams whose scores differ by less than some 1e-12 may come in either
+ * order, though in the same one for the same input.  A candidate whose 64-bit
+ * score is not finite is none (a row whose mask leaves nothing, or that holds a
+ * NaN or +inf at an allowed token, has none); slots that no candidate fills get
+ * score -inf, `pad`, their own index as parent, and count as finished.  A
+ * score below fp32's range is written as -inf, and the beam ends there.
  * next_scores may be scores and next_finished may be finished.  The workspace
  * (ng_beam_workspace bytes, 0 for many sizes) belongs to one call at a time. */
 size_t ng_beam_workspace(int groups, int beams, int vocab);

@@ -8,8 +8,9 @@
 // best, in order, are the next beams.
 //
 // The comparison between beams is one of sums of the same size, so lse and
-// totals are formed in 64 bits: which beam survives does not depend on how a
-// row was split over threads.  Within a beam the order of totals is the order
+// totals are formed in 64 bits, with exponentials good to 1e-12: which beam
+// survives does not depend on how a row was split over threads unless two
+// totals lie that close.  Within a beam the order of totals is the order
 // of logits, which needs no arithmetic: equal logits go to the lower token,
 // equal totals of two beams to the lower beam.
 //

@@ -70,7 +70,8 @@ __device__ __forceinline__ bool is_far(float v) {
 }
 
 // Sixteen consecutive bytes of a row from column k, zero past the row's end.
-// Rows start on 16-byte boundaries, so a chunk with one valid byte can be read.
+// Rows start on 16-byte boundaries, so a chunk with one valid byte can be read
+// whole: it lies in one aligned word, which no allocation ends within.
 __device__ __forceinline__ uint4 load16(const uint8_t *row, int k, int cols) {
   if (k >= cols) return make_uint4(0, 0, 0, 0);
   uint4 u = __ldg(reinterpret_cast<const uint4 *>(row + k));
@@ -212,9 +213,11 @@ __global__ void __launch_bounds__(32 * kVecWarps, CTAS) k_block_vec(BlockMatmulA
 // and nothing else.  A warp reads 64 columns at a time and gives a set back
 // before it adds the last of them.
 //
-// What bounds large products is the accumulators' way out: while MMAs run, one
-// of 128 x 256 takes some 700 clocks to read, and its own MMAs 541 (8192 x 8192
-// x 4096: 255 us, tensor pipe 56%).  Pairs of CTAs on one tile (cta_group::2)
+// What holds large products is the accumulators' way out: while MMAs run, one
+// of 128 x 256 is in registers some 700 clocks after it is ready, and its own
+// MMAs take 541 (8192 x 8192 x 4096: 251 us, tensor pipe 55%).  The 700 are
+// two loads of 64 columns a warp, the second issued as the first is added: the
+// marks do not tell TMEM's bandwidth from two of its latencies.  Pairs of CTAs on one tile (cta_group::2)
 // halve the weights' copies and not that, and hand back over the cluster, 500
 // clocks later: 512 us.
 //
@@ -905,7 +908,7 @@ template <int TN> void launch_tc(const BlockMatmulArgs &a, int splits, DeviceSet
 //   32 x 928 x 768     vec<2> 2.4 / 2.4, tc<32> 5.7 / 5.6    few tiles: latency
 //   256 x 768 x 3200   tc<64>, 4 splits 8.1 / 8.2, tc<32> 9.2 / 9.2
 //   1 x 8192 x 4096    vec<1> one block ahead 10.4 / 10.3, four ahead 13.9
-//   8192 x 8192 x 4096 tc<256> 253 / 255, tc<128> 316 / 320
+//   8192 x 8192 x 4096 tc<256> 253 / 251, tc<128> 316 / 320
 struct Plan {
   int vec; // rows of a a CTA of k_block_vec takes / 8; 0: k_block_tc with the two below
   int tn, splits;

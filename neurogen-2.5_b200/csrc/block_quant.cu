@@ -192,7 +192,7 @@ template <class T> __device__ __forceinline__ uint32_t amax_join(uint32_t a, uin
 
 // 1 x 128 blocks: few lanes a block, so that a block's scale and addresses cost
 // a fraction of a warp's instructions.  (8192 x 8192 bf16: a warp a block 103
-// us, eight lanes 38, four 33, 6.2 TB/s; 2048 x 6400 fp32 10.6 us, 6.2 TB/s.)
+// us, eight lanes 38, four 33, 6.2 TB/s; 2048 x 6400 fp32 10.0 us, 6.6 TB/s.)
 template <class T> constexpr int kRowLanes = sizeof(T) == 4 ? 8 : 4;
 
 template <class T, bool VEC> __global__ void __launch_bounds__(256) k_quant_rows(QuantArgs a, int kb, int blocks) {

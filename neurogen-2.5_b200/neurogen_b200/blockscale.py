@@ -3,8 +3,8 @@
 A matrix is e4m3 bytes with one fp32 scale for each block of 128 columns and one row
 (activations) or 128 rows (weights).  ``matmul`` multiplies two of them on the tensor cores; the
 engine's opt-in 8-bit projections (``NEUROGEN_PROJECTION=fp8``) are these operators.  They take
-CUDA tensors, run on the current stream of the tensors' device and do not synchronise; nothing
-is kept between calls.  Inference only: no gradients flow through them.
+CUDA tensors, run on the current stream of the tensors' device and do not synchronise; of a call's
+data nothing is kept.  Inference only: no gradients flow through them.
 """
 import torch
 

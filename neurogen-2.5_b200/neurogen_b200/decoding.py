@@ -25,10 +25,11 @@ def beam_select(logits, scores, finished=None, allowed=None, end=None, pad=PAD):
 
     Candidates are every beam's allowed tokens at score + log probability, and for a finished
     beam token ``pad`` at its own score.  A new beam is finished when its parent is or its token is
-    ``end``.  Scores are formed in 64 bits and rounded once; a beam's equal logits go to the lower
-    token, equal scores of two beams to the lower beam.  A candidate without a finite score is none; slots
-    that no candidate fills have score -inf, token ``pad``, their own index as parent, and count
-    as finished.  tokens and parents are int32; parents count within the group.
+    ``end``.  Scores are formed in 64 bits, from exponentials good to 1e-12, and rounded once; a beam's
+    equal logits go to the lower token, equal 64-bit scores of two beams to the lower beam (two within
+    some 1e-12 may come in either order, the same one for the same input).  A candidate without a finite
+    score is none; slots that no candidate fills have score -inf, token ``pad``, their own index as
+    parent, and count as finished.  tokens and parents are int32; parents count within the group.
     """
     rows, vocab = _matrix(logits, 'logits')
     code = ELEMENTS.get(logits.dtype)
